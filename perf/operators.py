@@ -355,7 +355,7 @@ def _leading(x, random_bits, codes):
 
 def _encode_m(x, random_bits):
     q, top, lowest, a = _leading(x, random_bits, 127)
-    up = x.abs() * 65536 > random_bits.float() * (lowest << 20).view(torch.float32)
+    up = x.abs() * 131072 > (2 * random_bits + 1).float() * (lowest << 20).view(torch.float32)
     k = torch.where(q >= lowest, q - (top - 127), torch.where(up, lowest - (top - 127), 0))
     return (k | torch.where((x < 0) & (k > 0), 128, 0)).to(torch.uint8), top.to(torch.int16)
 
