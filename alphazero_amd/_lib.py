@@ -39,6 +39,27 @@ class Stats(C.Structure):
                                           'games', 'errors')]
 
 
+class GroupNorm(C.Structure):
+    """az_group_norm"""
+    _fields_ = [('batch', C.c_int32), ('cells', C.c_int32), ('channels', C.c_int32), ('groups', C.c_int32),
+                ('dtype', C.c_int32), ('param_dtype', C.c_int32), ('act', C.c_int32), ('reserved', C.c_int32),
+                ('eps', C.c_double)]
+
+
+ADAMW_BLOCK, ADAMW_MAX_RUNS = 256, 32
+
+
+class AdamWRun(C.Structure):
+    """az_adamw_run"""
+    _fields_ = [('first_block', C.c_int64), ('half', C.c_int32), ('lr_index', C.c_int32), ('lr', C.c_double),
+                ('beta1', C.c_double), ('beta2', C.c_double), ('eps', C.c_double), ('weight_decay', C.c_double)]
+
+
+class AdamWBuffers(C.Structure):
+    """az_adamw_buffers"""
+    _fields_ = [(n, C.c_void_p) for n in ('p', 'g', 'p16', 'g16', 'm', 'v', 'm8', 'v8', 'top', 'step', 'arrived')]
+
+
 # every symbol include/azhip.h declares: name -> (restype, argtypes)
 _P = C.c_void_p
 SIGNATURES = {
@@ -103,6 +124,13 @@ SIGNATURES = {
     'az_c4net_pack_hx': (C.c_int, [_P, C.c_int32, C.c_double, _P, _P, _P]),
     'az_c4_train_fwd_bwd_chain': (C.c_int, [_P, _P, _P, _P, _P, C.c_int32, _P, _P, _P, _P, _P]),
     'az_c4_train_one_launch_max_batch': (C.c_int, [C.c_int32, _P]),
+    'az_group_norm_workspace_bytes': (C.c_int64, [C.POINTER(GroupNorm), C.c_int32]),
+    'az_group_norm_act': (C.c_int, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    'az_group_norm_act_backward': (C.c_int, [C.POINTER(GroupNorm), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    'az_adamw_step': (C.c_int, [C.POINTER(AdamWBuffers), C.c_int64, C.POINTER(AdamWRun), C.c_int32, C.c_int32, _P, C.c_uint64, _P,
+                                C.c_float, _P, _P]),
+    'az_adamw_decode8': (C.c_int, [_P, _P, _P, C.c_int64, _P, _P, _P]),
+    'az_adamw_encode8': (C.c_int, [_P, _P, C.c_int64, _P, _P, _P, _P]),
     'az_tttnet_f32_blob_floats': (C.c_int, [C.c_int32]),
     'az_tttnet_f32_forward': (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, C.c_int32, _P, _P, _P]),
 }

@@ -34,6 +34,13 @@ def _launch(device, fn):
         return check(fn(st))
 
 
+def _need_batch_norm(model):
+    """The kernels of this module fold batch-norm into the convolutions; a group-normalised network is evaluated by
+    calling the torch module."""
+    if getattr(model, 'norm', 'batch') != 'batch':
+        raise ValueError(f"the HIP networks are for norm='batch', got norm={model.norm!r}")
+
+
 def _fold_bn(w, bn, conv_bias=None):
     """Eval-mode BN folded into the preceding conv: returns (w * s[co], shift[co]) in float64."""
     s = bn.weight.double() / torch.sqrt(bn.running_var.double() + bn.eps)
@@ -120,6 +127,7 @@ def pack_c4_blob(model, out=None):
     given.  On a GPU it is one launch (az_c4net_pack_bf16), cheap enough to run after every optimiser step; a module on
     the CPU goes through the tensor operations of _pack_c4_blob_torch, which state the same layout and give the same
     bytes (tests/test_gpu_net.py)."""
+    _need_batch_norm(model)
     dev = model._cbr[0].weight.device
     if dev.type != 'cuda' or any(t.dtype != torch.float32 or not t.is_contiguous() for t in model.parameters()):
         blob = _pack_c4_blob_torch(model)
@@ -146,6 +154,7 @@ def pack_c4_blob(model, out=None):
 
 def _pack_c4_blob_torch(model):
     """The packed layout of csrc/az_net.hip stated in tensor operations (some 150 small launches on a GPU)."""
+    _need_batch_norm(model)
     C_ = model.block_channels
     if C_ > CMAX:
         raise ValueError(f'fused kernel supports up to {CMAX} trunk channels, got {C_}')
@@ -243,6 +252,7 @@ class FusedC4Net:
 def pack_c4_blob_f32(model):
     """AlphaZeroC4 module -> float32 tensor in the layout of csrc/az_net_f32.hip (BN folded in
     float64, then rounded once to float32)."""
+    _need_batch_norm(model)
     C_ = model.block_channels
     if C_ > CMAX or tuple(model.shape_in) != (2, 6, 7):
         raise ValueError('fused fp32 kernel: Connect Four nets with up to 32 trunk channels')
@@ -330,6 +340,7 @@ def pack_c4_blob_hx(model, out=None, range_error=None):
     launch (az_c4net_pack_hx); range_error = a device int32[1] that the launch sets when a folded weight does not fit
     fp16 (without it the call waits for the launch and raises, like the tensor statement _pack_c4_blob_hx_torch, which
     a module on the CPU goes through and which gives the same bytes)."""
+    _need_batch_norm(model)
     dev = model._cbr[0].weight.device
     if dev.type != 'cuda' or any(t.dtype != torch.float32 or not t.is_contiguous() for t in model.parameters()):
         blob = _pack_c4_blob_hx_torch(model)
@@ -360,6 +371,7 @@ def pack_c4_blob_hx(model, out=None, range_error=None):
 
 def _pack_c4_blob_hx_torch(model):
     """The packed layout of csrc/az_net_hx_dev.h stated in tensor operations."""
+    _need_batch_norm(model)
     C_ = model.block_channels
     if C_ > CMAX or tuple(model.shape_in) != (2, 6, 7):
         raise ValueError('fp16-pair kernel: Connect Four nets with up to 32 trunk channels')
@@ -447,6 +459,7 @@ class FusedC4NetHX:
 
 def pack_c4_blob_128(model):
     """AlphaZeroC4 with 128 trunk channels -> uint8 blob in the layout of csrc/az_net128.hip."""
+    _need_batch_norm(model)
     if model.block_channels != 128 or tuple(model.shape_in) != (2, 6, 7):
         raise ValueError('az_net128 is for Connect Four nets with 128 trunk channels')
     dev = model._cbr[0].weight.device
@@ -515,6 +528,7 @@ TTT_WIDTHS = (4, 8, 16)      # trunk channels of the tic-tac-toe kernel (csrc/az
 def pack_ttt_blob_f32(model):
     """AlphaZero module with shape_in (2,3,3), shape_out (9,) -> float32 tensor in the layout of
     csrc/az_net_ttt.hip (BN folded in float64, then rounded once to float32)."""
+    _need_batch_norm(model)
     C_ = model.block_channels
     if tuple(model.shape_in) != (2, 3, 3) or tuple(model.shape_out) != (9,) or C_ not in TTT_WIDTHS:
         raise ValueError('tic-tac-toe kernel: shape_in (2,3,3), shape_out (9,), 4, 8 or 16 trunk channels')
@@ -566,7 +580,7 @@ class TTTNetF32:
 
     @classmethod
     def supports(cls, model):
-        return (getattr(model, 'shape_in', None) == (2, 3, 3) and getattr(model, 'shape_out', None) == (9,)
+        return (getattr(model, 'norm', 'batch') == 'batch' and getattr(model, 'shape_in', None) == (2, 3, 3) and getattr(model, 'shape_out', None) == (9,)
                 and getattr(model, 'block_channels', None) in TTT_WIDTHS)
 
     def load_module(self, model):

@@ -88,7 +88,9 @@ class SelfPlayWorker:
             # evaluated by calling the torch module on the rendered leaves
             from .models import AlphaZero, AlphaZeroC4
             from .net import CMAX, C4Net128, FusedC4Net, FusedC4NetHX, TTTNetF32
-            if isinstance(self._model, AlphaZeroC4) and self._model.block_channels <= CMAX:
+            if getattr(self._model, 'norm', 'batch') != 'batch':
+                pass                      # (the kernels fold batch-norm: a group-normalised network runs as the torch module)
+            elif isinstance(self._model, AlphaZeroC4) and self._model.block_channels <= CMAX:
                 self._fused = (FusedC4NetHX(self._model, self._device) if net_precision == 'fp32'
                                else FusedC4Net.from_module(self._model, self._device))
             elif isinstance(self._model, AlphaZeroC4) and self._model.block_channels == 128:

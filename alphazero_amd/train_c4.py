@@ -67,7 +67,7 @@ def supports(model):
     """True for the network these kernels are written for: AlphaZeroC4 (2x6x7 -> 6x7) with 32 trunk channels, default
     batch-norm settings, on a GPU."""
     from .models import AlphaZeroC4
-    if not isinstance(model, AlphaZeroC4) or model.block_channels != 32:
+    if not isinstance(model, AlphaZeroC4) or model.block_channels != 32 or model.norm != 'batch':
         return False
     bns = [m for m in model.modules() if isinstance(m, torch.nn.BatchNorm2d)]
     if any(m.momentum is None or not m.affine or not m.track_running_stats for m in bns):

@@ -1,5 +1,6 @@
 """TrainingWorker with the reference's constructor and process_batch() contract
-(alphazero/training.py:15-125): SGD + momentum + weight decay, MultiStepLR, masked
+(alphazero/training.py:15-125): SGD + momentum + weight decay (or, with `training.optimizer: adamw`, AdamW:
+optim.FlatAdamW, csrc/az_adamw.hip), MultiStepLR, masked
 cross-entropy + MSE, weights published after every step.  On the GPU the loss with its gradients and the
 optimiser update are hand-written kernels (loss.AlphaZeroLoss, optim.FlatSGD; csrc/az_train.hip).  For the
 Connect Four network with 32 trunk channels the whole pass -- forward on the batch's statistics, loss, backward,
@@ -36,7 +37,23 @@ class TrainingWorker:
         self._model = config.Model().to(device)
         self._loss = config.Loss()
         t = config.training
-        if torch.device(device).type == 'cuda':
+        # training.optimizer: 'sgd' as the reference (the default), or 'adamw' with betas, eps, state_bits (32, or 8 on
+        # the GPU) and seed
+        kind = t.get('optimizer', 'sgd')
+        if kind not in ('sgd', 'adamw'):
+            raise ValueError(f"training.optimizer is 'sgd' or 'adamw', got {kind!r}")
+        if kind == 'adamw':
+            kwargs = dict(lr=t['lr'], betas=tuple(t.get('betas', (0.9, 0.999))), eps=float(t.get('eps', 1e-8)),
+                          weight_decay=t['weight_decay'])
+            if torch.device(device).type == 'cuda':
+                from .optim import FlatAdamW
+                self._optimizer = FlatAdamW(self._model.parameters(), state_bits=t.get('state_bits', 32),
+                                            seed=t.get('seed', 0), **kwargs)
+            else:
+                if t.get('state_bits', 32) != 32:
+                    raise ValueError('training.state_bits: moments in 8 bits need a GPU')
+                self._optimizer = torch.optim.AdamW(self._model.parameters(), **kwargs)
+        elif torch.device(device).type == 'cuda':
             # one launch per step over a flat parameter buffer (csrc/az_train.hip)
             from .optim import FlatSGD
             self._optimizer = FlatSGD(self._model.parameters(), lr=t['lr'], momentum=t['momentum'],

@@ -452,6 +452,79 @@ int  az_sgd_momentum_guarded(float* params, const float* grads, float* momentum_
                              float momentum, float weight_decay, const float* guard_dev, float guard_limit,
                              int32_t* withheld_dev, void* stream);
 
+/* ---- group norm with an activation and a residual sum, channels last ----------------------------------------
+ * What a residual tower without batch statistics puts where the reference has nn.BatchNorm2d + ReLU
+ * (alphazero/models.py:6-28): x [batch][cells][channels] (channels last: a cell's channels lie together),
+ *   z = (x - mean) * rstd * weight[c] + bias[c] (+ residual),  y = act(z),
+ * mean and rstd = 1 / sqrt(var + eps) over the cells and the channels / groups channels of a sample's group; sums and
+ * statistics in 64 bits, the rest in 32, one rounding to the tensors' type.  relu and its gradient pass a NaN on.
+ * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any size and alignment
+ * (16-byte aligned tensors and groups of a multiple of 4 channels, 8 in 16 bits, run fastest).                    */
+#define AZ_F32  0
+#define AZ_BF16 1
+#define AZ_F16  2
+#define AZ_ACT_NONE 0
+#define AZ_ACT_RELU 1   /* z <= 0 ? 0 : z           */
+#define AZ_ACT_SILU 2   /* z / (1 + exp(-z))        */
+typedef struct az_group_norm {
+    int32_t batch, cells, channels, groups;      /* batch may be 0; channels divide by groups */
+    int32_t dtype, param_dtype;                  /* AZ_F32, AZ_BF16 or AZ_F16                 */
+    int32_t act, reserved;
+    double  eps;
+} az_group_norm;
+/* bytes of DEVICE workspace a call needs, forward or backward (contents need not be kept between calls and need no
+ * initialisation; two calls that may run at the same time need one each; 16-byte aligned); -1 for a bad descriptor */
+int64_t az_group_norm_workspace_bytes(const az_group_norm* g, int32_t backward);
+/* DEVICE pointers.  weight, bias (1 and 0 when NULL), residual and stats may be NULL; stats double[batch][groups][2] =
+ * {mean, rstd} is what the backward call reads.  y may not overlap x or residual.  No allocation, no host
+ * synchronisation (both calls can be recorded in a HIP graph).                                                    */
+int  az_group_norm_act(const az_group_norm* g, const void* x, const void* weight, const void* bias, const void* residual,
+                       void* y, double* stats, void* workspace, int64_t workspace_bytes, void* stream);
+/* The gradients of sum(dy * y): dx, dweight, dbias, dresidual, each of them written unless NULL.  x, weight, bias,
+ * residual and stats as in the forward call.  Sums over the batch are added in a fixed order: the same inputs give the
+ * same bits.                                                                                                      */
+int  az_group_norm_act_backward(const az_group_norm* g, const void* dy, const void* x, const void* weight, const void* bias,
+                                const void* residual, const double* stats, void* dx, void* dweight, void* dbias,
+                                void* dresidual, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- AdamW over all tensors of a network in one launch --------------------------------------------------------
+ * Beside az_sgd_momentum (the reference's optimiser, alphazero/training.py:27-29).  Tensors lie behind each other in
+ * flat buffers, each from a multiple of AZ_ADAMW_BLOCK elements on, the gaps zero; tensors that share their settings
+ * form a run of blocks.  Per element, t = step[0] + 1:
+ *   m = (beta1 * m) + ((1 - beta1) * g);  v = (beta2 * v) + ((1 - beta2) * (g * g));
+ *   p = p * (1 - lr * weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * p is float32 everywhere; in a run with half != 0 the parameters and gradients are bfloat16 (p16, g16) and p is their
+ * master copy, p16 its rounding (a p16 that is not was written by somebody else, and the master becomes it).  state_bits 32: m, v float32.  state_bits 8: m8, v8 one byte per element and
+ * top uint16[blocks][2], 11 leading float bits of each block's largest |m| and v (format and rounding: csrc/az_adamw.hip);
+ * they are rounded at random by bits that are a function of (seed, t, element), so the same call gives the same bits
+ * on every rank.  step DEVICE int64[1] counts the updates applied; arrived DEVICE int32[1] starts as zero and is
+ * zero after every call.  All buffers are 16-byte aligned.  One call at a time may use the same buffers.           */
+#define AZ_ADAMW_BLOCK 256
+#define AZ_ADAMW_MAX_RUNS 32
+typedef struct az_adamw_run {
+    int64_t first_block;                         /* ascending; the first run begins at 0 */
+    int32_t half, lr_index;
+    double  lr, beta1, beta2, eps, weight_decay;
+} az_adamw_run;
+typedef struct az_adamw_buffers {                /* what a call does not use may be NULL */
+    float* p; const float* g;
+    uint16_t* p16; const uint16_t* g16;
+    float* m; float* v;
+    uint8_t* m8; uint8_t* v8; uint16_t* top;
+    int64_t* step; int32_t* arrived;
+} az_adamw_buffers;
+/* lr_dev: NULL, or DEVICE double[] whose entry lr_index takes the place of a run's lr when the kernel runs (for launches
+ * recorded in a HIP graph, as az_sgd_momentum_lr_dev).  guard_dev, guard_limit, withheld_dev: NULL, or the check of
+ * az_sgd_momentum_guarded: unless guard_dev[0] < guard_limit nothing is written, the step count included, and
+ * withheld_dev[0] is incremented.                                                                                  */
+int  az_adamw_step(const az_adamw_buffers* b, int64_t blocks, const az_adamw_run* runs, int32_t num_runs, int32_t state_bits,
+                   const double* lr_dev, uint64_t seed, const float* guard_dev, float guard_limit, int32_t* withheld_dev,
+                   void* stream);
+/* moments in 8 bits -> the float32 values they stand for, and back.  Values that came from codes come back as the same
+ * values; others are rounded to the nearest.                                                                       */
+int  az_adamw_decode8(const uint8_t* m8, const uint8_t* v8, const uint16_t* top, int64_t blocks, float* m, float* v, void* stream);
+int  az_adamw_encode8(const float* m, const float* v, int64_t blocks, uint8_t* m8, uint8_t* v8, uint16_t* top, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
