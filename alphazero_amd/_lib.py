@@ -46,7 +46,7 @@ class GroupNorm(C.Structure):
                 ('eps', C.c_double)]
 
 
-ADAMW_BLOCK, ADAMW_MAX_RUNS = 256, 32
+ADAMW_BLOCK, ADAMW_MAX_RUNS, ADAMW_STEPS = 256, 32, 16384
 
 
 class AdamWRun(C.Structure):
@@ -57,7 +57,7 @@ class AdamWRun(C.Structure):
 
 class AdamWBuffers(C.Structure):
     """az_adamw_buffers"""
-    _fields_ = [(n, C.c_void_p) for n in ('p', 'g', 'p16', 'g16', 'm', 'v', 'm8', 'v8', 'top', 'step', 'arrived')]
+    _fields_ = [(n, C.c_void_p) for n in ('p', 'g', 'p16', 'g16', 'm', 'v', 'm8', 'v8', 'top', 'step')]
 
 
 # every symbol include/azhip.h declares: name -> (restype, argtypes)
@@ -166,3 +166,12 @@ def check(rc):
 def ptr(t):
     """Device (or host) pointer of a torch tensor / None."""
     return None if t is None else C.c_void_p(t.data_ptr())
+
+
+def launch(device, fn, *args):
+    """check(fn(*args, stream)) on the current stream of `device`, with `device` current."""
+    import torch
+    if torch.cuda.current_device() == device.index:
+        return check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    with torch.cuda.device(device):
+        return check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))

@@ -52,14 +52,6 @@ def _workspace(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _call(device, fn, args):
-    """fn(*args, stream) with `device` current."""
-    if torch.cuda.current_device() == device.index:
-        return _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
-    with torch.cuda.device(device):
-        return _lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
-
-
 def _last(t):
     """Channels last, without a copy where it is that already."""
     if t.dim() == 2:
@@ -80,8 +72,8 @@ def _forward(x, num_groups, weight, bias, eps, act, residual, keep):
     y = torch.empty_like(x)
     stats = torch.empty(x.shape[0], num_groups, 2, dtype=torch.float64, device=x.device) if keep else None
     ws = _workspace(d[1], x.device)
-    _call(x.device, _lib.load().az_group_norm_act,
-          (d[0], x.data_ptr(), _at(weight), _at(bias), _at(residual), y.data_ptr(), _at(stats), _at(ws), d[1]))
+    _lib.launch(x.device, _lib.load().az_group_norm_act, d[0], x.data_ptr(), _at(weight), _at(bias), _at(residual), y.data_ptr(),
+                _at(stats), _at(ws), d[1])
     return y, d, stats
 
 
@@ -104,9 +96,8 @@ class _GroupNormAct(torch.autograd.Function):
         db = torch.empty_like(bias) if needs[2] else None
         dr = torch.empty_like(residual) if needs[3] else None
         ws = _workspace(d[2], x.device)
-        _call(x.device, _lib.load().az_group_norm_act_backward,
-              (d[0], dy.data_ptr(), x.data_ptr(), _at(weight), _at(bias), _at(residual), stats.data_ptr(),
-               _at(dx), _at(dw), _at(db), _at(dr), _at(ws), d[2]))
+        _lib.launch(x.device, _lib.load().az_group_norm_act_backward, d[0], dy.data_ptr(), x.data_ptr(), _at(weight), _at(bias),
+                    _at(residual), stats.data_ptr(), _at(dx), _at(dw), _at(db), _at(dr), _at(ws), d[2])
         return dx, dw, db, dr, None, None, None
 
 

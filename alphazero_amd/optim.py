@@ -142,7 +142,7 @@ class FlatAdamW(torch.optim.Optimizer):
         for _, _, p in order:
             if p.device != dev or p.dtype not in (torch.float32, torch.bfloat16) or p.layout != torch.strided:
                 raise ValueError(f'FlatAdamW takes dense float32 or bfloat16 parameters on one device, got {p.dtype} on {p.device}')
-        self.lib, self.device = _lib.load(), dev
+        self.lib, self.device = _lib.load(), dev           # (a parameter's device has its index)
         self._runs, self._places, block = [], [], 0
         for k, half, p in order:
             if not self._runs or (self._runs[-1][0], self._runs[-1][1]) != (k, half):
@@ -166,7 +166,7 @@ class FlatAdamW(torch.optim.Optimizer):
         else:
             self.codes_m, self.codes_v = zeros(torch.uint8), zeros(torch.uint8)
             self.tops = zeros(torch.int16, 2 * block)
-        self._step_dev, self._arrived = zeros(torch.int64, 1), zeros(torch.int32, 1)
+        self._step_dev = zeros(torch.int64, _lib.ADAMW_STEPS)   # a counter for each workgroup, all equal
         self.withheld = zeros(torch.int32, 1)              # recorded steps whose update the guard refused
         self._lr_dev, self._lr_host = None, None
         self._grads = []
@@ -188,7 +188,7 @@ class FlatAdamW(torch.optim.Optimizer):
         b = _lib.AdamWBuffers()
         for name, t in (('p', self.flat_p), ('g', self.flat_g), ('p16', self.flat_p16), ('g16', self.flat_g16), ('m', self.flat_m),
                         ('v', self.flat_v), ('m8', self.codes_m), ('v8', self.codes_v), ('top', self.tops),
-                        ('step', self._step_dev), ('arrived', self._arrived)):
+                        ('step', self._step_dev)):
             setattr(b, name, None if t is None else t.data_ptr())
         self._buffers = b
         self._args = (_lib.AdamWRun * len(self._runs))()
@@ -216,7 +216,7 @@ class FlatAdamW(torch.optim.Optimizer):
     @property
     def steps(self):
         """Updates applied so far (waits for the device)."""
-        return int(self._step_dev.item())
+        return int(self._step_dev[0].item())
 
     def zero_grad(self, set_to_none=False):
         for flat in (self.flat_g, self.flat_g16):          # the .grad views stay in place
@@ -235,20 +235,17 @@ class FlatAdamW(torch.optim.Optimizer):
                 if p.grad is None:
                     raise _lib.AzError('a parameter of FlatAdamW has no gradient: use its own zero_grad(), which keeps the '
                                        'gradients in place')
-                grad.copy_(p.grad)
+                with torch.no_grad():
+                    grad.copy_(p.grad)
                 p.grad = grad
 
     def _launch(self, lr_dev, guard, guard_limit):
         for a, (k, _, _) in zip(self._args, self._runs):
             g = self.param_groups[k]
             a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = g['lr'], g['betas'], g['eps'], g['weight_decay']
-        with torch.cuda.device(self.device):
-            st = torch.cuda.current_stream(self.device).cuda_stream
-            _lib.check(self.lib.az_adamw_step(self._buffers, self._blocks, self._args, len(self._runs), self.state_bits,
-                                              _lib.ptr(lr_dev), self.seed, _lib.ptr(guard), float(guard_limit),
-                                              _lib.ptr(self.withheld), st))
+        _lib.launch(self.device, self.lib.az_adamw_step, self._buffers, self._blocks, self._args, len(self._runs), self.state_bits,
+                    _lib.ptr(lr_dev), self.seed, _lib.ptr(guard), guard_limit, self.withheld.data_ptr())
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -269,7 +266,6 @@ class FlatAdamW(torch.optim.Optimizer):
                 self._lr_dev[k].fill_(lr)
         self._lr_host = rates
 
-    @torch.no_grad()
     def step_recorded(self, guard=None, guard_limit=1e-6):
         """The same update with the learning rates read from device memory at run time, for launches captured in a HIP
         graph; the other settings are those of the capture.  Call set_recorded_lr() (outside the capture) before every
@@ -287,10 +283,8 @@ class FlatAdamW(torch.optim.Optimizer):
         if self.state_bits == 32:
             return self.flat_m, self.flat_v
         m, v = torch.empty_like(self.flat_p), torch.empty_like(self.flat_p)
-        with torch.cuda.device(self.device):
-            st = torch.cuda.current_stream(self.device).cuda_stream
-            _lib.check(self.lib.az_adamw_decode8(_lib.ptr(self.codes_m), _lib.ptr(self.codes_v), _lib.ptr(self.tops), self._blocks,
-                                                 _lib.ptr(m), _lib.ptr(v), st))
+        _lib.launch(self.device, self.lib.az_adamw_decode8, self.codes_m.data_ptr(), self.codes_v.data_ptr(), self.tops.data_ptr(),
+                    self._blocks, m.data_ptr(), v.data_ptr())
         return m, v
 
     def state_dict(self):
@@ -332,8 +326,6 @@ class FlatAdamW(torch.optim.Optimizer):
             if p.dtype == torch.bfloat16:
                 self._cut(self.flat_p, p, at).copy_(p if e is None or 'master' not in e else e['master'])
         if self.state_bits == 8:
-            with torch.cuda.device(self.device):
-                st = torch.cuda.current_stream(self.device).cuda_stream
-                _lib.check(self.lib.az_adamw_encode8(_lib.ptr(m), _lib.ptr(v), self._blocks, _lib.ptr(self.codes_m),
-                                                     _lib.ptr(self.codes_v), _lib.ptr(self.tops), st))
+            _lib.launch(self.device, self.lib.az_adamw_encode8, m.data_ptr(), v.data_ptr(), self._blocks, self.codes_m.data_ptr(),
+                        self.codes_v.data_ptr(), self.tops.data_ptr())
         self._step_dev.fill_(steps.pop())

@@ -490,17 +490,18 @@ int  az_group_norm_act_backward(const az_group_norm* g, const void* dy, const vo
 /* ---- AdamW over all tensors of a network in one launch --------------------------------------------------------
  * Beside az_sgd_momentum (the reference's optimiser, alphazero/training.py:27-29).  Tensors lie behind each other in
  * flat buffers, each from a multiple of AZ_ADAMW_BLOCK elements on, the gaps zero; tensors that share their settings
- * form a run of blocks.  Per element, t = step[0] + 1:
+ * form a run of blocks.  Per element, t = step + 1:
  *   m = (beta1 * m) + ((1 - beta1) * g);  v = (beta2 * v) + ((1 - beta2) * (g * g));
  *   p = p * (1 - lr * weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * p is float32 everywhere; in a run with half != 0 the parameters and gradients are bfloat16 (p16, g16) and p is their
  * master copy, p16 its rounding (a p16 that is not was written by somebody else, and the master becomes it).  state_bits 32: m, v float32.  state_bits 8: m8, v8 one byte per element and
  * top uint16[blocks][2], 11 leading float bits of each block's largest |m| and v (format and rounding: csrc/az_adamw.hip);
  * they are rounded at random by bits that are a function of (seed, t, element), so the same call gives the same bits
- * on every rank.  step DEVICE int64[1] counts the updates applied; arrived DEVICE int32[1] starts as zero and is
- * zero after every call.  All buffers are 16-byte aligned.  One call at a time may use the same buffers.           */
+ * on every rank.  step DEVICE int64[AZ_ADAMW_STEPS] counts the updates applied (one counter for each workgroup: set all to
+ * the same number, step[0] is the count).  All buffers are 16-byte aligned.  One call at a time may use the same buffers. */
 #define AZ_ADAMW_BLOCK 256
 #define AZ_ADAMW_MAX_RUNS 32
+#define AZ_ADAMW_STEPS 16384
 typedef struct az_adamw_run {
     int64_t first_block;                         /* ascending; the first run begins at 0 */
     int32_t half, lr_index;
@@ -511,7 +512,7 @@ typedef struct az_adamw_buffers {                /* what a call does not use may
     uint16_t* p16; const uint16_t* g16;
     float* m; float* v;
     uint8_t* m8; uint8_t* v8; uint16_t* top;
-    int64_t* step; int32_t* arrived;
+    int64_t* step;
 } az_adamw_buffers;
 /* lr_dev: NULL, or DEVICE double[] whose entry lr_index takes the place of a run's lr when the kernel runs (for launches
  * recorded in a HIP graph, as az_sgd_momentum_lr_dev).  guard_dev, guard_limit, withheld_dev: NULL, or the check of

@@ -90,7 +90,8 @@ def _check(got, want, tol, dtype, param):
 
 SHAPES = [(1, 256, 32, 6, 7), (5, 2, 1, 6, 7), (3, 1, 1, 3, 3), (2, 30, 5, 5, 3), (4, 12, 3, 1, 1), (7, 64, 64, 4, 4), (130, 128, 16, 6, 7),
           (2, 1300, 1, 3, 3), (1, 2200, 2, 2, 2), (2, 64, 8, 32, 32), (1, 320, 32, 64, 64), (3, 48, 4, 19, 19), (9, 16, 1, 3, 3),
-          (33, 8, 1, 1, 5), (1, 1, 1, 1, 1), (300, 24, 8, 6, 7), (2, 96, 1, 61, 3), (600, 4, 2, 1, 1), (3, 20, 1, 50, 41), (1, 512, 2, 40, 40)]
+          (33, 8, 1, 1, 5), (1, 1, 1, 1, 1), (300, 24, 8, 6, 7), (2, 96, 1, 61, 3), (600, 4, 2, 1, 1), (3, 20, 1, 50, 41), (1, 512, 2, 40, 40),
+          (2, 6000, 1, 2, 3), (3, 2051, 1, 3, 3), (2, 60, 6, 48, 31), (70, 128, 16, 20, 20)]
 
 
 @pytest.mark.parametrize('shape', SHAPES)

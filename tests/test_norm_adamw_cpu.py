@@ -108,7 +108,7 @@ def test_c_entries_refuse_null_pointers_and_small_workspaces():
 
 def test_adamw_c_entries_refuse_bad_arguments():
     lib = _lib.load()
-    b = _lib.AdamWBuffers(*([1 << 12] * 11))
+    b = _lib.AdamWBuffers(*([1 << 12] * 10))
     run = lambda **kw: _lib.AdamWRun(**dict(dict(first_block=0, half=0, lr_index=0, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8), **kw))
     call = lambda b, n, runs, bits, **kw: lib.az_adamw_step(
         b, n, (_lib.AdamWRun * max(len(runs), 1))(*runs), len(runs), bits, kw.get('lr_dev'), 0, kw.get('guard'), 0.0, None, None)
@@ -120,14 +120,14 @@ def test_adamw_c_entries_refuse_bad_arguments():
                               (4, [run()], 32, dict(guard=4096))]:
         assert call(b, n, runs, bits, **kw) != 0, (n, bits, kw)
         assert b'az_adamw_step' in lib.az_last_error()
-    for k, bits in (('p', 32), ('g', 32), ('m', 32), ('v', 32), ('m8', 8), ('v8', 8), ('top', 8), ('step', 32), ('arrived', 8)):
-        short = _lib.AdamWBuffers(*([1 << 12] * 11))
+    for k, bits in (('p', 32), ('g', 32), ('m', 32), ('v', 32), ('m8', 8), ('v8', 8), ('top', 8), ('step', 32)):
+        short = _lib.AdamWBuffers(*([1 << 12] * 10))
         setattr(short, k, None)
         assert call(short, 4, [run()], bits) != 0 and b'null' in lib.az_last_error(), k
-    short = _lib.AdamWBuffers(*([1 << 12] * 11))
+    short = _lib.AdamWBuffers(*([1 << 12] * 10))
     short.g16 = None
     assert call(short, 4, [run(half=1)], 32) != 0 and b'null' in lib.az_last_error()
-    odd = _lib.AdamWBuffers(*([1 << 12] * 11))
+    odd = _lib.AdamWBuffers(*([1 << 12] * 10))
     odd.m = (1 << 12) + 4
     assert call(odd, 4, [run()], 32) != 0 and b'aligned' in lib.az_last_error()
     assert lib.az_adamw_decode8(None, None, None, 1, None, None, None) != 0
