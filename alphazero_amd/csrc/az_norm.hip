@@ -31,7 +31,7 @@ struct GnArgs {
     long N;
     int HW, C, G, Cg, cpg;            // cpg: vectors per group
     int cb, gb, rb, sb, tb;           // held samples: bits of column, group, row, sample in a team's thread; of the team
-    int gs, cw, rstep;                // others: groups of a slice, vectors of a group (or piece of one), rows of a workgroup
+    int gs, cw, rstep, share;         // others: groups of a slice, vectors of a group (or piece of one), rows of a workgroup
     int slices, pieces, chunks, rows; // rows per chunk
     int together;                     // slices share lines of memory
     int walkers;                      // teams that share a slice's samples in the backward pass
@@ -169,81 +169,103 @@ __device__ __forceinline__ void gn_moments(double s, double q, const GnArgs& a, 
     rstd = y * fma(-0.5 * v * y, y, 1.5);
 }
 
+// (addresses: a scalar base, the same for a wave, and 32 bits of a lane's own; two registers an address and vector otherwise)
+template <typename T, int VW> __device__ __forceinline__ typename GnVec<T, VW>::type gn_raw(const void* base, long at, uint32_t lane) {
+    return *reinterpret_cast<const typename GnVec<T, VW>::type*>(reinterpret_cast<const char*>(base) + at + lane);
+}
+template <typename T, int VW> __device__ __forceinline__ void gn_get(const void* base, long at, uint32_t lane, float (&out)[VW]) {
+    gn_load<T, VW>(reinterpret_cast<const char*>(base) + at + lane, 0, out);
+}
+template <typename T, int VW> __device__ __forceinline__ void gn_put(void* base, long at, uint32_t lane, const float (&in)[VW]) {
+    gn_store<T, VW>(reinterpret_cast<char*>(base) + at + lane, 0, in);
+}
+
 // ---- samples too large for registers: two passes over chunks of their rows -------------------------------------------
 // A workgroup has a slice (gs groups; or a piece of one that is wider than 256 vectors) of a chunk of a sample's rows, its
 // threads side by side along memory: thread = row * gs * cw + group * cw + column.  First pass: sums; second: the rest,
 // whose every workgroup adds the parts of its groups up again.
+// Workgroups go to the card's 8 dies in turn; where the slices of a sample share lines of memory, neighbours in this
+// numbering are on one die, whose L2 then fetches a line once.
+__device__ __forceinline__ unsigned gn_block(const GnArgs& a) {
+    const unsigned b = blockIdx.x, die = b & 7, per = gridDim.x >> 3, more = gridDim.x & 7;
+    return a.together ? die * per + min(die, more) + (b >> 3) : b;
+}
+
 struct GnPlace {
-    long n; int g, gl, col, row, chunk, piece, width; bool on;
-    long base;                        // element of its first channel in row 0
+    long n; int g, gl, col, row, chunk, piece, width, rows; bool on;
+    long base;                        // bytes to the chunk: the same for the workgroup
+    uint32_t lane, step;              // bytes on to this thread's first row, and to its next
 };
 
-__device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int VW) {
+__device__ __forceinline__ GnPlace gn_place(const GnArgs& a, int VW, int size) {
     GnPlace p;
-    unsigned u = blockIdx.x;
-    p.chunk = u % a.chunks; u /= a.chunks;
+    unsigned u = gn_block(a);
+    const int slice = u % a.slices, t = threadIdx.x; u /= a.slices;
     p.piece = u % a.pieces; u /= a.pieces;
-    const int slice = u % a.slices, t = threadIdx.x;
-    p.n = u / a.slices;
+    p.chunk = u % a.chunks;
+    p.n = u / a.chunks;
     p.width = a.gs * a.cw;
     p.row = t / p.width;
     p.gl = t % p.width / a.cw;
     p.col = t % a.cw + p.piece * a.cw;
     p.g = slice * a.gs + p.gl;
     p.on = p.row < a.rstep && p.col < a.cpg && p.g < a.G;
-    p.base = p.n * a.HW * a.C + (long)p.g * a.Cg + (long)p.col * VW;
+    p.rows = min(a.rows, a.HW - p.chunk * a.rows);
+    p.base = (p.n * a.HW + (long)p.chunk * a.rows) * a.C * size;
+    p.lane = ((uint32_t)p.row * a.C + p.g * a.Cg + p.col * VW) * size;
+    p.step = (uint32_t)a.rstep * a.C * size;
     return p;
 }
 
-// (s, q) over the threads of each group -> the workgroup's entry of that group's parts
+// (s, q) over the threads of each group -> the workgroup's entry of that group's parts; a.share neighbouring threads add
+// for a group
 __device__ __forceinline__ void gn_put_parts(const GnArgs& a, const GnPlace& p, double s, double q, double (*lds)[2]) {
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, gl = t / a.share, g = p.g - p.gl + gl;
     lds[t][0] = s; lds[t][1] = q;
     __syncthreads();
-    if (t < p.width)
-        for (int r = 1; r < a.rstep; ++r) { s += lds[r * p.width + t][0]; q += lds[r * p.width + t][1]; }
-    __syncthreads();
-    if (t < p.width) { lds[t][0] = s; lds[t][1] = q; }
-    __syncthreads();
-    const int g = p.g - p.gl + t;
-    if (t < a.gs && g < a.G) {
-        s = q = 0.0;
-        for (int c = 0; c < a.cw; ++c) { s += lds[t * a.cw + c][0]; q += lds[t * a.cw + c][1]; }
+    s = q = 0.0;
+    if (gl < a.gs)
+        for (int k = t % a.share; k < a.rstep * a.cw; k += a.share) {
+            const int from = k / a.cw * p.width + gl * a.cw + k % a.cw;
+            s += lds[from][0]; q += lds[from][1];
+        }
+    gn_wave_sum(s, q, a.share - 1);
+    if (gl < a.gs && g < a.G && t % a.share == 0) {
         double* out = a.part + ((p.n * a.G + g) * (a.pieces * a.chunks) + p.piece * a.chunks + p.chunk) * 2;
         out[0] = s; out[1] = q;
     }
 }
 
-// the sums of the parts of this thread's group, in order; at most 16 threads add for a group, then one
+// the sums of the parts of this thread's group, in order
 __device__ __forceinline__ void gn_get_parts(const GnArgs& a, const GnPlace& p, double& s, double& q, double (*lds)[2]) {
-    const int t = threadIdx.x, parts = a.pieces * a.chunks, share = min(16, GN_THREADS / a.gs);
-    const int gl = t / share, g = p.g - p.gl + gl;
+    const int t = threadIdx.x, parts = a.pieces * a.chunks, gl = t / a.share, g = p.g - p.gl + gl;
     s = q = 0.0;
     if (gl < a.gs && g < a.G) {
         const double* in = a.part + (p.n * a.G + g) * parts * 2;
-        for (int k = t % share; k < parts; k += share) { s += in[2 * k]; q += in[2 * k + 1]; }
+        for (int k = t % a.share; k < parts; k += a.share) { s += in[2 * k]; q += in[2 * k + 1]; }
     }
-    lds[t][0] = s; lds[t][1] = q;
+    gn_wave_sum(s, q, a.share - 1);
+    if (t % a.share == 0) { lds[gl][0] = s; lds[gl][1] = q; }
     __syncthreads();
-    s = q = 0.0;
-    for (int k = 0; k < share; ++k) { s += lds[p.gl * share + k][0]; q += lds[p.gl * share + k][1]; }
+    s = lds[p.gl][0]; q = lds[p.gl][1];
 }
 
 template <typename T, int VW>
 __global__ void __launch_bounds__(GN_THREADS)
 k_gn_stats(GnArgs a) {
     __shared__ double lds[GN_THREADS][2];
-    const GnPlace p = gn_place(a, VW);
+    const GnPlace p = gn_place(a, VW, sizeof(T));
     double s = 0.0, q = 0.0;
-    const int r1 = min(a.HW, (p.chunk + 1) * a.rows);
-    if (p.on)
+    if (p.on) {
+        uint32_t at = p.lane;
 #pragma unroll 4
-        for (int r = p.chunk * a.rows + p.row; r < r1; r += a.rstep) {
+        for (int r = p.row; r < p.rows; r += a.rstep, at += p.step) {
             float x[VW];
-            gn_load<T, VW>(a.x, p.base + (long)r * a.C, x);
+            gn_get<T, VW>(a.x, p.base, at, x);
 #pragma unroll
             for (int i = 0; i < VW; ++i) { const double d = x[i]; s += d; q = fma(d, d, q); }
         }
+    }
     gn_put_parts(a, p, s, q, lds);
 }
 
@@ -285,7 +307,7 @@ template <typename T, int VW, bool SILU>
 __global__ void __launch_bounds__(GN_THREADS)
 k_gn_apply(GnArgs a) {
     __shared__ double lds[GN_THREADS][2];
-    const GnPlace p = gn_place(a, VW);
+    const GnPlace p = gn_place(a, VW, sizeof(T));
     double s, q, mean, rstd;
     gn_get_parts(a, p, s, q, lds);
     if (!p.on) return;
@@ -299,25 +321,23 @@ k_gn_apply(GnArgs a) {
     gn_param<VW>(a.w, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 1.0f, w);
     gn_param<VW>(a.b, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 0.0f, b);
     gn_affine<VW>(k, w, b);
-    const int r1 = min(a.HW, (p.chunk + 1) * a.rows);
     constexpr int U = GN_ROWS(VW);
-    for (int r0 = p.chunk * a.rows + p.row; r0 < r1; r0 += U * a.rstep) {
+    uint32_t at = p.lane;
+    for (int r0 = p.row; r0 < p.rows; r0 += U * a.rstep, at += U * p.step) {
         float x[U][VW], z[U][VW] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * a.rstep;
-            if (r < r1) {
-                gn_load<T, VW>(a.x, p.base + (long)r * a.C, x[u]);
-                if (a.res) gn_load<T, VW>(a.res, p.base + (long)r * a.C, z[u]);
+            if (r0 + u * a.rstep < p.rows) {
+                gn_get<T, VW>(a.x, p.base, at + u * p.step, x[u]);
+                if (a.res) gn_get<T, VW>(a.res, p.base, at + u * p.step, z[u]);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * a.rstep;
-            if (r < r1) {
+            if (r0 + u * a.rstep < p.rows) {
 #pragma unroll
                 for (int i = 0; i < VW; ++i) z[u][i] = gn_act<SILU>(fmaf(x[u][i] - k.mh, w[i], b[i]) + z[u][i], a.low);
-                gn_store<T, VW>(a.y, p.base + (long)r * a.C, z[u]);
+                gn_put<T, VW>(a.y, p.base, at + u * p.step, z[u]);
             }
         }
     }
@@ -367,7 +387,7 @@ __global__ void __launch_bounds__(GN_THREADS)
 k_gn_bwd_sums(GnArgs a) {
     __shared__ double lds[GN_THREADS][2];
     __shared__ float sums[2 * VW][GN_THREADS];
-    const GnPlace p = gn_place(a, VW);
+    const GnPlace p = gn_place(a, VW, sizeof(T));
     double sa = 0.0, sx = 0.0;
     float dw[VW] = {}, db[VW] = {};
     if (p.on) {
@@ -375,23 +395,21 @@ k_gn_bwd_sums(GnArgs a) {
         float w[VW], b[VW];
         gn_param<VW>(a.w, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 1.0f, w);
         gn_param<VW>(a.b, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 0.0f, b);
-        const int r1 = min(a.HW, (p.chunk + 1) * a.rows);
         constexpr int U = GN_ROWS(VW);
-        for (int r0 = p.chunk * a.rows + p.row; r0 < r1; r0 += U * a.rstep) {
+        uint32_t at = p.lane;
+        for (int r0 = p.row; r0 < p.rows; r0 += U * a.rstep, at += U * p.step) {
             float x[U][VW], dy[U][VW], res[U][VW] = {};
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * a.rstep;
-                if (r < r1) {
-                    gn_load<T, VW>(a.x, p.base + (long)r * a.C, x[u]);
-                    gn_load<T, VW>(a.dy, p.base + (long)r * a.C, dy[u]);
-                    if (a.res) gn_load<T, VW>(a.res, p.base + (long)r * a.C, res[u]);
+                if (r0 + u * a.rstep < p.rows) {
+                    gn_get<T, VW>(a.x, p.base, at + u * p.step, x[u]);
+                    gn_get<T, VW>(a.dy, p.base, at + u * p.step, dy[u]);
+                    if (a.res) gn_get<T, VW>(a.res, p.base, at + u * p.step, res[u]);
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int r = r0 + u * a.rstep;
-                if (r < r1) {
+                if (r0 + u * a.rstep < p.rows) {
                     gn_dz_row<VW, SILU>(a, k, x[u], w, b, res[u], dy[u]);
                     float fa = 0.0f, fx = 0.0f;
 #pragma unroll
@@ -403,7 +421,7 @@ k_gn_bwd_sums(GnArgs a) {
                         fx = fmaf(f, xhat, fx);
                     }
                     sa += fa; sx += fx;
-                    if (a.dres) gn_store<T, VW>(a.dres, p.base + (long)r * a.C, dy[u]);
+                    if (a.dres) gn_put<T, VW>(a.dres, p.base, at + u * p.step, dy[u]);
                 }
             }
         }
@@ -427,7 +445,7 @@ template <typename T, int VW, bool SILU>
 __global__ void __launch_bounds__(GN_THREADS)
 k_gn_bwd_apply(GnArgs a) {
     __shared__ double lds[GN_THREADS][2];
-    const GnPlace p = gn_place(a, VW);
+    const GnPlace p = gn_place(a, VW, sizeof(T));
     double sa, sx;
     gn_get_parts(a, p, sa, sx, lds);
     if (!p.on) return;
@@ -436,29 +454,27 @@ k_gn_bwd_apply(GnArgs a) {
     float w[VW], b[VW];
     gn_param<VW>(a.w, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 1.0f, w);
     gn_param<VW>(a.b, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 0.0f, b);
-    const int r1 = min(a.HW, (p.chunk + 1) * a.rows);
     // what the first pass wrote as the residual's gradient is dz, except where silu's was rounded to 16 bits
     const bool have = a.dres && (!SILU || sizeof(T) == 4);
     constexpr int U = GN_ROWS(VW);
-    for (int r0 = p.chunk * a.rows + p.row; r0 < r1; r0 += U * a.rstep) {
+    uint32_t at = p.lane;
+    for (int r0 = p.row; r0 < p.rows; r0 += U * a.rstep, at += U * p.step) {
         float x[U][VW], dy[U][VW], res[U][VW] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * a.rstep;
-            if (r < r1) {
-                gn_load<T, VW>(a.x, p.base + (long)r * a.C, x[u]);
-                gn_load<T, VW>(have ? a.dres : a.dy, p.base + (long)r * a.C, dy[u]);
-                if (a.res && !have) gn_load<T, VW>(a.res, p.base + (long)r * a.C, res[u]);
+            if (r0 + u * a.rstep < p.rows) {
+                gn_get<T, VW>(a.x, p.base, at + u * p.step, x[u]);
+                gn_get<T, VW>(have ? a.dres : a.dy, p.base, at + u * p.step, dy[u]);
+                if (a.res && !have) gn_get<T, VW>(a.res, p.base, at + u * p.step, res[u]);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int r = r0 + u * a.rstep;
-            if (r < r1) {
+            if (r0 + u * a.rstep < p.rows) {
                 if (!have) gn_dz_row<VW, SILU>(a, k, x[u], w, b, res[u], dy[u]);
 #pragma unroll
                 for (int i = 0; i < VW; ++i) dy[u][i] = (fmaf(dy[u][i], w[i], -ma) - gn_xhat(k, x[u][i]) * mx) * k.rs;
-                gn_store<T, VW>(a.dx, p.base + (long)r * a.C, dy[u]);
+                gn_put<T, VW>(a.dx, p.base, at + u * p.step, dy[u]);
             }
         }
     }
@@ -496,23 +512,9 @@ k_gn_dparams(const float* __restrict__ dpart, long parts, int C, int wtype, void
 // A thread holds VW neighbouring channels of one group in each of its rows.  The bits of its index in the team are, from
 // the lowest: column within the group (cb), group within the slice (gb), row (rb), sample (sb).  Sums over a group are
 // butterflies over the column and row bits, so a wave's loads run along memory whatever the group's width.
-// (addresses: a scalar base, the same for a wave, and 32 bits of a lane's own; two registers an address and vector otherwise)
-template <typename T, int VW> __device__ __forceinline__ typename GnVec<T, VW>::type gn_raw(const void* base, long at, uint32_t lane) {
-    return *reinterpret_cast<const typename GnVec<T, VW>::type*>(reinterpret_cast<const char*>(base) + at + lane);
-}
-template <typename T, int VW> __device__ __forceinline__ void gn_put(void* base, long at, uint32_t lane, const float (&in)[VW]) {
-    gn_store<T, VW>(reinterpret_cast<char*>(base) + at + lane, 0, in);
-}
 template <typename T, int VW> __device__ __forceinline__ float gn_at(const typename GnVec<T, VW>::type& v, int i) {
     if constexpr (VW == 1) return (float)v;
     else return (float)v[i];
-}
-
-// Workgroups go to the card's 8 dies in turn; where the slices of a sample share lines of memory, neighbours in this
-// numbering are on one die, whose L2 then fetches a line once.
-__device__ __forceinline__ unsigned gn_block(const GnArgs& a) {
-    const unsigned b = blockIdx.x, die = b & 7, per = gridDim.x >> 3, more = gridDim.x & 7;
-    return a.together ? die * per + min(die, more) + (b >> 3) : b;
 }
 
 struct GnSeat { int col, gl, row, sample; };
@@ -753,8 +755,8 @@ static GnArgs gn_plan(const az_group_norm* g, int VW) {
     a.pieces = (a.cpg + a.cw - 1) / a.cw;
     a.gs = 1;
     if (a.pieces == 1) {
-        // groups side by side: 128 bytes of a row at least, then the fewest idle threads
-        const int line = 128 / (VW * gn_size(g->dtype)), most = a.G < GN_THREADS / a.cw ? a.G : GN_THREADS / a.cw;
+        // groups side by side: 64 bytes of a row at least, then the fewest idle threads
+        const int line = 64 / (VW * gn_size(g->dtype)), most = a.G < GN_THREADS / a.cw ? a.G : GN_THREADS / a.cw;
         int low = (line + a.cw - 1) / a.cw;
         if (low > most) low = most;
         long best = -1;
@@ -765,14 +767,19 @@ static GnArgs gn_plan(const az_group_norm* g, int VW) {
         }
     }
     a.rstep = GN_THREADS / (a.gs * a.cw);
+    for (a.share = 16; a.share * a.gs > GN_THREADS; a.share >>= 1) {}
     a.slices = (a.G + a.gs - 1) / a.gs;
-    // rows in chunks while there are too few workgroups to fill the card, four rows of a thread at least
+    a.together = (int64_t)a.gs * a.Cg * gn_size(g->dtype) % 128 != 0;
+    // Rows in chunks while there are too few workgroups to fill the card, four rows of a thread at least; every chunk of the
+    // second pass reads the parts of all, so not too many (3 x 4096 cells x 320 channels, bfloat16, forward: 13.4 us with up
+    // to 32, 15.2 with up to 128)
     const long units = a.N * a.slices * a.pieces;
     long chunks = units ? (1024 + units - 1) / units : 1;
     const long most = (a.HW + 4 * a.rstep - 1) / (4 * a.rstep);
     if (chunks > most) chunks = most;
-    if (chunks > 64) chunks = 64;
-    if (chunks < 1) chunks = 1;
+    if (chunks > 32) chunks = 32;
+    const long least = ((long)a.HW * a.C * gn_size(g->dtype) >> 31) + 1;         // (a chunk's offsets in 32 bits)
+    if (chunks < least) chunks = least;
     a.rows = (int)((a.HW + chunks - 1) / chunks);
     a.chunks = (a.HW + a.rows - 1) / a.rows;
     return a;
