@@ -158,6 +158,25 @@ def load():
     return lib
 
 
+_autograd = None
+AUTOGRAD_ENTRIES = ('az_last_error', 'az_group_norm_workspace_bytes', 'az_group_norm_act', 'az_group_norm_act_backward')
+
+
+def autograd():
+    """The autograd functions of csrc/az_torch.cpp, bound to the library that load() has loaded."""
+    global _autograd
+    if _autograd is None:
+        lib = load()
+        try:
+            from . import _az_torch
+        except ImportError as e:
+            raise AzError(f'alphazero_amd/_az_torch.so: {e}: build it with `make -C alphazero_amd/csrc torch` '
+                          '(python -c "import __graft_entry__ as g; g.build()")') from e
+        _az_torch.bind([C.cast(getattr(lib, n), C.c_void_p).value for n in AUTOGRAD_ENTRIES])
+        _autograd = _az_torch
+    return _autograd
+
+
 def check(rc):
     if rc != 0:
         raise AzError(load().az_last_error().decode())

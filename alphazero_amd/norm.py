@@ -4,11 +4,9 @@ no statistics of the batch, so a network is the same function in training, in se
 
     y = act((x - mean) * rstd * weight + bias + residual)      mean, rstd over a sample's group of channels
 
-On the GPU forward and backward are hand-written kernels (no fallback there: a missing library raises); CPU tensors
-take the torch statement below."""
-import ctypes as C
+On the GPU forward and backward are hand-written kernels behind an autograd function (csrc/az_torch.cpp; no fallback
+there: a missing library raises); CPU tensors take the torch statement below."""
 import math
-from functools import lru_cache
 
 import torch
 from torch import nn
@@ -16,7 +14,7 @@ from torch import nn
 from . import _lib
 
 ACTS = {'none': 0, 'relu': 1, 'silu': 2}
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _statement(x, num_groups, weight, bias, eps, act, residual):
@@ -36,69 +34,11 @@ def _statement(x, num_groups, weight, bias, eps, act, residual):
     return z.to(x.dtype)
 
 
-@lru_cache(maxsize=4096)
-def _descriptor(n, cells, channels, groups, dtype, param_dtype, act, eps):
-    """(az_group_norm, forward workspace bytes, backward workspace bytes): functions of the sizes alone."""
-    lib = _lib.load()
-    g = _lib.GroupNorm(n, cells, channels, groups, dtype, param_dtype, act, 0, eps)
-    sizes = [lib.az_group_norm_workspace_bytes(C.byref(g), k) for k in (0, 1)]
-    if min(sizes) < 0:
-        raise _lib.AzError(lib.az_last_error().decode())
-    return (g, *sizes)
-
-
-def _workspace(nbytes, device):
-    # one for each call, from torch's allocator: calls on several streams or in several captured graphs share nothing
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
 def _last(t):
     """Channels last, without a copy where it is that already."""
     if t.dim() == 2:
         return t.contiguous()
     return t.contiguous(memory_format=torch.channels_last)
-
-
-def _at(t):
-    return None if t is None else t.data_ptr()
-
-
-def _forward(x, num_groups, weight, bias, eps, act, residual, keep):
-    """y, the descriptor and (if `keep`) the statistics the backward pass reads; x and residual channels last."""
-    cells = x.shape[2] * x.shape[3] if x.dim() == 4 else 1
-    param = weight if weight is not None else bias
-    d = _descriptor(x.shape[0], cells, x.shape[1], num_groups, DTYPES[x.dtype], 0 if param is None else DTYPES[param.dtype],
-                    ACTS[act], eps)
-    y = torch.empty_like(x)
-    stats = torch.empty(x.shape[0], num_groups, 2, dtype=torch.float64, device=x.device) if keep else None
-    ws = _workspace(d[1], x.device)
-    _lib.launch(x.device, _lib.load().az_group_norm_act, d[0], x.data_ptr(), _at(weight), _at(bias), _at(residual), y.data_ptr(),
-                _at(stats), _at(ws), d[1])
-    return y, d, stats
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, num_groups, eps, act):
-        y, ctx.descriptor, stats = _forward(x, num_groups, weight, bias, eps, act, residual, True)
-        ctx.save_for_backward(x, weight, bias, residual, stats)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, residual, stats = ctx.saved_tensors
-        needs = ctx.needs_input_grad
-        d = ctx.descriptor
-        dy = _last(dy)
-        dx = torch.empty_like(x) if needs[0] else None
-        dw = torch.empty_like(weight) if needs[1] else None
-        db = torch.empty_like(bias) if needs[2] else None
-        dr = torch.empty_like(residual) if needs[3] else None
-        ws = _workspace(d[2], x.device)
-        _lib.launch(x.device, _lib.load().az_group_norm_act_backward, d[0], dy.data_ptr(), x.data_ptr(), _at(weight), _at(bias),
-                    _at(residual), stats.data_ptr(), _at(dx), _at(dw), _at(db), _at(dr), _at(ws), d[2])
-        return dx, dw, db, dr, None, None, None
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act='relu', residual=None):
@@ -135,9 +75,7 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act='relu', 
     residual = None if residual is None else _last(residual)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return _GroupNormAct.apply(x, weight, bias, residual, num_groups, eps, act)
-    return _forward(x, num_groups, weight, bias, eps, act, residual, False)[0]
+    return _lib.autograd().group_norm_act(x, weight, bias, residual, num_groups, eps, ACTS[act])
 
 
 class GroupNormAct(nn.GroupNorm):

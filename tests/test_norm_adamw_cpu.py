@@ -201,3 +201,11 @@ def test_training_worker_takes_the_optimizer_from_the_config():
     for bad in (dict(optimizer='lamb'), dict(optimizer='adamw', state_bits=8)):
         with pytest.raises(ValueError):
             TrainingWorker(_config(**bad), None, Window(), None, 'cpu')
+
+
+def test_autograd_functions_are_bound_to_the_loaded_library():
+    m = _lib.autograd()
+    assert m is _lib.autograd() and callable(m.group_norm_act)
+    with pytest.raises(RuntimeError, match='four entry points'):
+        m.bind([])
+    assert _lib.autograd() is m
