@@ -28,9 +28,10 @@
 
 #define ADAMW_BLOCK 256          // elements: four of each lane of a wave
 // A wave takes a block, four neighbouring elements to a lane, so that every load and store of a wave is one piece of memory.
-// Bound by memory (28 bytes an element in 32 bits, 16 in 8): 46 M parameters 222 us = 5.8 TB/s and 132 us = 5.6 TB/s, a copy
-// of the same size 4.7 to 5.2.  Workgroups of 512 threads that take one block a wave and end: their traffic moves along
-// memory as one front.  2048 workgroups that walk over the blocks: 238 to 250 and 137 to 146 us.
+// Bound by memory in 32 bits (28 bytes an element): 46 M parameters 222 us = 5.8 TB/s, where a copy of as much has 4.7 to 5.2.
+// In 8 bits (16 bytes) by memory and instructions alike: 129 us = 5.7 TB/s, and some 110 instructions an element, a quarter
+// of them the random numbers.  Workgroups of 512 threads that take one block a wave and end: their traffic moves along memory as
+// one front.  2048 workgroups that walk over the blocks: 238 to 250 and 137 to 146 us.
 #define ADAMW_THREADS 512
 #define ADAMW_GOLDEN 0x9E3779B97F4A7C15ull
 
@@ -136,6 +137,31 @@ __device__ __forceinline__ f32x4 adamw_values_v(uint32_t codes, int top) {
 template <typename T> __device__ __forceinline__ T adamw_load(const void* p) { return __builtin_nontemporal_load(reinterpret_cast<const T*>(p)); }
 template <typename T> __device__ __forceinline__ void adamw_store(void* p, const T& v) { __builtin_nontemporal_store(v, reinterpret_cast<T*>(p)); }
 
+// what a lane reads of a block
+template <int BITS> struct AdamwIn {
+    f32x4 p, g, m, v;
+    bf16x4 h, p16;                    // bfloat16 runs: gradient and parameter
+    uint32_t m8, v8, top;
+};
+
+template <int BITS>
+__device__ __forceinline__ void adamw_read(const az_adamw_buffers& q, long blk, int lane, int half, AdamwIn<BITS>& in) {
+    const long at = blk * ADAMW_BLOCK + lane * 4;
+    in.p = *reinterpret_cast<const f32x4*>(q.p + at);
+    if (half) {
+        in.h = adamw_load<bf16x4>(q.g16 + at);
+        in.p16 = *reinterpret_cast<const bf16x4*>(q.p16 + at);
+    } else in.g = adamw_load<f32x4>(q.g + at);
+    if constexpr (BITS == 32) {
+        in.m = adamw_load<f32x4>(q.m + at);
+        in.v = adamw_load<f32x4>(q.v + at);
+    } else {
+        in.m8 = adamw_load<uint32_t>(q.m8 + at);
+        in.v8 = adamw_load<uint32_t>(q.v8 + at);
+        in.top = *reinterpret_cast<const uint32_t*>(q.top + 2 * blk);
+    }
+}
+
 template <int BITS>
 __global__ void __launch_bounds__(ADAMW_THREADS)
 k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restrict__ lr_dev, uint64_t seed,
@@ -146,7 +172,17 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
     }
     __shared__ AdamwScalars sc[AZ_ADAMW_MAX_RUNS];
     const int tid = threadIdx.x, lane = tid & 63;
+    const long stride = (long)gridDim.x * (ADAMW_THREADS / 64);
+    long blk = (long)blockIdx.x * (ADAMW_THREADS / 64) + __builtin_amdgcn_readfirstlane(tid >> 6);
+    int run = 0;
+    // the first block is on its way while the scalars are made (two functions in 64 bits; 1.2 M parameters in 32 bits:
+    // 7.9 -> 6.7 us)
+    AdamwIn<BITS> in;
     const int64_t t = q.step[blockIdx.x] + 1;
+    if (blk < blocks) {
+        while (run + 1 < runs.n && blk >= runs.r[run + 1].first_block) ++run;
+        adamw_read<BITS>(q, blk, lane, runs.r[run].half, in);
+    }
     if (tid < runs.n) {
         const AdamwRun& r = runs.r[tid];
         const double lr = lr_dev ? lr_dev[r.lr_index] : r.lr;
@@ -162,29 +198,21 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
     __syncthreads();
     if (tid == 0) q.step[blockIdx.x] = t;                                 // (behind the barrier: every thread has read it)
     const uint64_t key = adamw_mix(seed + ADAMW_GOLDEN * (uint64_t)t);
-    const int waves = ADAMW_THREADS / 64;
-    int run = 0;
-    for (long blk = (long)blockIdx.x * waves + __builtin_amdgcn_readfirstlane(tid >> 6); blk < blocks; blk += (long)gridDim.x * waves) {
-        while (run + 1 < runs.n && blk >= runs.r[run + 1].first_block) ++run;
+    while (blk < blocks) {
         const AdamwScalars s = sc[run];
         const long at = blk * ADAMW_BLOCK + lane * 4;
-        f32x4 p = *reinterpret_cast<const f32x4*>(q.p + at), g, m, v;
+        f32x4 p = in.p, g, m, v;
         if (s.half) {
-            const bf16x4 h = adamw_load<bf16x4>(q.g16 + at);
-            const bf16x4 cur = *reinterpret_cast<const bf16x4*>(q.p16 + at);
-            g = __builtin_convertvector(h, f32x4);
+            g = __builtin_convertvector(in.h, f32x4);
             // a parameter that is not its master's rounding was written by somebody else (a checkpoint loaded): it counts
-            const u16x4 have = __builtin_bit_cast(u16x4, cur), mine = __builtin_bit_cast(u16x4, __builtin_convertvector(p, bf16x4));
+            const u16x4 have = __builtin_bit_cast(u16x4, in.p16), mine = __builtin_bit_cast(u16x4, __builtin_convertvector(p, bf16x4));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = have[i] != mine[i] ? (float)cur[i] : p[i];
-        } else g = adamw_load<f32x4>(q.g + at);
-        if constexpr (BITS == 32) {
-            m = adamw_load<f32x4>(q.m + at);
-            v = adamw_load<f32x4>(q.v + at);
-        } else {
-            const uint32_t cm = adamw_load<uint32_t>(q.m8 + at), cv = adamw_load<uint32_t>(q.v8 + at);
-            m = adamw_values_m(cm, q.top[2 * blk]);
-            v = adamw_values_v(cv, q.top[2 * blk + 1]);
+            for (int i = 0; i < 4; ++i) p[i] = have[i] != mine[i] ? (float)in.p16[i] : p[i];
+        } else g = in.g;
+        if constexpr (BITS == 32) { m = in.m; v = in.v; }
+        else {
+            m = adamw_values_m(in.m8, in.top & 0xFFFFu);
+            v = adamw_values_v(in.v8, in.top >> 16);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -212,6 +240,11 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
             adamw_store(q.m8 + at, adamw_codes_m(m, adamw_mix(counter), tm));
             adamw_store(q.v8 + at, adamw_codes_v(v, adamw_mix(counter + ADAMW_GOLDEN), tv));
             if (lane == 0) *reinterpret_cast<uint32_t*>(q.top + 2 * blk) = (uint32_t)tm | ((uint32_t)tv << 16);
+        }
+        blk += stride;
+        if (blk < blocks) {
+            while (run + 1 < runs.n && blk >= runs.r[run + 1].first_block) ++run;
+            adamw_read<BITS>(q, blk, lane, runs.r[run].half, in);
         }
     }
 }

@@ -105,7 +105,7 @@ class FlatAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW (decoupled weight decay, bias correction; no amsgrad) with the whole update of all parameter
     groups in ONE launch of az_adamw_step (csrc/az_adamw.hip), beside FlatSGD.
 
-    All parameters that require gradients move into one flat buffer (each becomes a view of it, padded to 256
+    All parameters that require gradients at construction move into one flat buffer (each becomes a view of it, padded to 256
     elements), gradients accumulate into a second through persistent `.grad` views (use this class's zero_grad; a
     gradient that was replaced by another tensor is copied back into its view).  Parameters are float32, or bfloat16
     with a float32 master copy that the update works on (weights written between two steps, as by
@@ -203,6 +203,8 @@ class FlatAdamW(torch.optim.Optimizer):
             raise ValueError(f'betas lie in [0, 1), got {g["betas"]}')
         if not (g['lr'] >= 0.0 and g['eps'] >= 0.0 and g['weight_decay'] >= 0.0):
             raise ValueError('lr, eps and weight_decay are not negative')
+        if g.get('amsgrad') or g.get('maximize'):
+            raise ValueError('FlatAdamW has no amsgrad and no maximize')
 
     @staticmethod
     def _cut(flat, p, at):
@@ -242,7 +244,7 @@ class FlatAdamW(torch.optim.Optimizer):
     def _launch(self, lr_dev, guard, guard_limit):
         for a, (k, _, _) in zip(self._args, self._runs):
             g = self.param_groups[k]
-            a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = g['lr'], g['betas'], g['eps'], g['weight_decay']
+            a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = float(g['lr']), g['betas'], g['eps'], g['weight_decay']
         _lib.launch(self.device, self.lib.az_adamw_step, self._buffers, self._blocks, self._args, len(self._runs), self.state_bits,
                     _lib.ptr(lr_dev), self.seed, _lib.ptr(guard), guard_limit, self.withheld.data_ptr())
 
@@ -313,9 +315,9 @@ class FlatAdamW(torch.optim.Optimizer):
         for (p, _), e in zip(self._places, entries):
             if e is not None and (e['exp_avg'].shape != p.shape or e['exp_avg_sq'].shape != p.shape):
                 raise ValueError(f'moments of shape {tuple(e["exp_avg"].shape)} for a parameter of shape {tuple(p.shape)}')
-        super().load_state_dict(dict(state_dict, state={}))
-        for g in self.param_groups:
+        for g in state_dict['param_groups']:
             self._check_group(g)
+        super().load_state_dict(dict(state_dict, state={}))
         m, v = (self.flat_m, self.flat_v) if self.state_bits == 32 else (torch.zeros_like(self.flat_p), torch.zeros_like(self.flat_p))
         m.zero_()
         v.zero_()

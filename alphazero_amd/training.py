@@ -43,7 +43,7 @@ class TrainingWorker:
         if kind not in ('sgd', 'adamw'):
             raise ValueError(f"training.optimizer is 'sgd' or 'adamw', got {kind!r}")
         if kind == 'adamw':
-            kwargs = dict(lr=t['lr'], betas=tuple(t.get('betas', (0.9, 0.999))), eps=float(t.get('eps', 1e-8)),
+            kwargs = dict(lr=t['lr'], betas=tuple(float(b) for b in t.get('betas', (0.9, 0.999))), eps=float(t.get('eps', 1e-8)),
                           weight_decay=t['weight_decay'])
             if torch.device(device).type == 'cuda':
                 from .optim import FlatAdamW

@@ -498,7 +498,8 @@ int  az_group_norm_act_backward(const az_group_norm* g, const void* dy, const vo
  * top uint16[blocks][2], 11 leading float bits of each block's largest |m| and v (format and rounding: csrc/az_adamw.hip);
  * they are rounded at random by bits that are a function of (seed, t, element), so the same call gives the same bits
  * on every rank.  step DEVICE int64[AZ_ADAMW_STEPS] counts the updates applied (one counter for each workgroup: set all to
- * the same number, step[0] is the count).  All buffers are 16-byte aligned.  One call at a time may use the same buffers. */
+ * the same number, step[0] is the count; `blocks` is the same in every call with the same counters).  All buffers are
+ * 16-byte aligned.  One call at a time may use the same buffers.                                                    */
 #define AZ_ADAMW_BLOCK 256
 #define AZ_ADAMW_MAX_RUNS 32
 #define AZ_ADAMW_STEPS 16384

@@ -331,13 +331,14 @@ def test_bad_state_is_refused():
     sd = opt.state_dict()
     before = opt.state_values()[0].clone()
     for spoil in (lambda s: s['state'].pop(0), lambda s: s['state'][0].update(step=7), lambda s: s['state'][0].update(exp_avg=torch.zeros(3)),
-                  lambda s: s['param_groups'][0].update(betas=(1.0, 0.9))):
+                  lambda s: s['param_groups'][0].update(betas=(1.0, 0.9)), lambda s: s['param_groups'][0].update(amsgrad=True)):
         bad = opt.state_dict()
         spoil(bad)
         with pytest.raises(ValueError):
             opt.load_state_dict(bad)
-        opt.load_state_dict(sd)
-        assert torch.equal(opt.state_values()[0], before) and opt.steps == 1
+        assert torch.equal(opt.state_values()[0], before) and opt.steps == 1 and opt.param_groups[0]['betas'] == (0.9, 0.999)
+    opt.load_state_dict(sd)
+    assert torch.equal(opt.state_values()[0], before) and opt.steps == 1
 
 
 @pytest.mark.parametrize('bits', [8, 32])

@@ -354,3 +354,72 @@ def test_autocast_keeps_the_convolutions_type():
     (p.float().sum() + v.float().sum()).backward()
     assert kinds == [(torch.bfloat16, True)] * 3
     assert all(q.grad is not None and bool(q.grad.isfinite().all()) for q in m.parameters())
+
+
+def _draws(count):
+    import random
+    rng = random.Random(2)
+    for _ in range(count):
+        groups, per = rng.choice([1, 2, 3, 4, 5, 8, 16, 32, 33]), rng.choice([1, 2, 3, 4, 6, 7, 8, 10, 12, 16, 24, 40])
+        h, w = rng.choice([(1, 1), (3, 3), (6, 7), (1, 13), (19, 19), (rng.randint(1, 48), rng.randint(1, 48))])
+        n = rng.randint(1, max(1, min(700, 400000 // (groups * per * h * w))))
+        yield n, groups * per, groups, h, w, rng.choice(list(DT)), rng.choice(['none', 'relu', 'silu']), rng.random() < 0.5, rng.random() < 0.3
+
+
+@pytest.mark.parametrize('n,c,groups,h,w,dtype,act,residual,off', list(_draws(120)))
+def test_drawn_shapes_write_their_own_values_only(n, c, groups, h, w, dtype, act, residual, off):
+    """Through the C entry points, outputs in the middle of buffers of a pattern that has to survive (`off`: also one
+    value off any 16-byte border), the workspace exactly as large as asked for and between patterns too."""
+    import ctypes as C
+    from alphazero_amd import _lib
+    lib, dt = _lib.load(), DT[dtype]
+    x, wt, b, r, dy = _inputs(n, c, h, w, dt, torch.float32, residual, seed=n + c + h)
+    g = _lib.GroupNorm(n, h * w, c, groups, ['f32', 'bf16', 'f16'].index(dtype), 0, ['none', 'relu', 'silu'].index(act), 0, 1e-5)
+    pad, banks = 4096, []
+
+    def bank(count, kind):
+        buf = torch.full((count + 2 * pad + 8,), 7.0, dtype=kind, device='cuda') if kind.is_floating_point else torch.full(
+            (count + 2 * pad + 8,), 77, dtype=kind, device='cuda')
+        at = pad + (1 if off and kind == dt else 0)
+        banks.append((buf, at, count))
+        return buf[at:at + count]
+    y, dx, dr = (bank(x.numel(), dt) for _ in range(3))
+    dw, db = bank(c, torch.float32), bank(c, torch.float32)
+    stats = bank(2 * n * groups, torch.float64)
+    sizes = [lib.az_group_norm_workspace_bytes(C.byref(g), k) for k in (0, 1)]
+    ws = [bank(s, torch.uint8) for s in sizes]
+    p = lambda t: None if t is None else t.data_ptr()
+    st = torch.cuda.current_stream().cuda_stream
+    _lib.check(lib.az_group_norm_act(C.byref(g), p(x), p(wt), p(b), p(r), p(y), p(stats), p(ws[0]) if sizes[0] else None, sizes[0], st))
+    _lib.check(lib.az_group_norm_act_backward(C.byref(g), p(dy), p(x), p(wt), p(b), p(r), p(stats), p(dx), p(dw), p(db),
+                                              p(dr) if residual else None, p(ws[1]) if sizes[1] else None, sizes[1], st))
+    torch.cuda.synchronize()
+    for buf, at, count in banks:
+        rest = torch.cat([buf[:at], buf[at + count:]])
+        assert bool((rest == (7.0 if buf.dtype.is_floating_point else 77)).all()), (buf.dtype, count)
+    if not residual:
+        assert bool((dr == 7.0).all())
+    want, tol = _reference(x, groups, wt, b, r, dy, act)
+    cells = lambda t: t.reshape(n, h, w, c).permute(0, 3, 1, 2)
+    got = dict(y=cells(y), dx=cells(dx), dw=dw, db=db)
+    if residual:
+        got['dr'] = cells(dr)
+    _check(got, want, tol, dt, torch.float32)
+
+
+def test_a_graph_kept_and_run_twice_and_inference_mode():
+    from alphazero_amd.norm import group_norm_act
+    x, wt, b, r, dy = _inputs(9, 24, 6, 7, torch.float32, torch.float32, True, 17)
+    leaves = [t.detach().requires_grad_() for t in (x, wt, b, r)]
+    y = group_norm_act(leaves[0], 3, leaves[1], leaves[2], residual=leaves[3])
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(p, q) and p.data_ptr() != q.data_ptr() for p, q in zip(first, again))
+    with torch.inference_mode():
+        assert torch.equal(group_norm_act(x, 3, wt, b, residual=r), y)
+    leaves[0].data.add_(0)                                         # (data: no new version)
+    y = group_norm_act(leaves[0] * 1, 3, leaves[1], leaves[2])
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
