@@ -159,6 +159,8 @@ class TrainingWorker:
             self._optimizer.zero_grad()
             total = policy_loss + value_loss
             total.backward()
+            # a writer may keep what it is given: no graph of the parameters may live on when the step is recorded
+            policy_loss, value_loss, total = policy_loss.detach(), value_loss.detach(), total.detach()
         if self._grad_sync is not None:
             self._grad_sync(self._model)
         self._optimizer.step()

@@ -534,6 +534,26 @@ def test_training_worker_with_group_norm_and_adamw(norm, bits):
         assert (a - b).abs().max() <= 10 * 3 * 1e-3 * (0.125 if bits == 8 else 0.01)
 
 
+def test_a_writer_may_keep_what_it_is_given():
+    """The losses of the eager steps, kept as tensors, hold no graph of the parameters when the step is recorded."""
+    from alphazero_amd.training import TrainingWorker
+
+    class Keeper:
+        kept = []
+
+        def add_scalar(self, tag, value, step):
+            self.kept.append(value)
+    dev = torch.device('cuda:0')
+    tw = TrainingWorker(_job('group', 32), _Server(), _window(dev), Keeper(), dev)
+    for _ in range(tw.EAGER_STEPS):
+        tw.process_batch()
+    tensors = [v for v in Keeper.kept if torch.is_tensor(v)]
+    assert tensors and all(v.grad_fn is None for v in tensors)
+    for _ in range(3):
+        tw.process_batch()
+    assert tw._graph is not None and tw._optimizer.steps == 6
+
+
 def test_recorded_step_of_a_bad_batch_is_withheld():
     from alphazero_amd.training import TrainingWorker
     dev = torch.device('cuda:0')
