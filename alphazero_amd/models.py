@@ -106,6 +106,8 @@ class AlphaZero(nn.Module):
         self._tower = nn.Sequential(*([shared] * num_blocks))
         self._policy_head = PolicyHead((block_channels, *shape_in[1:]), shape_out, norm)
         self._value_head = ValueHead((block_channels, *shape_in[1:]), norm)
+        if norm == 'group':
+            self.to(memory_format=torch.channels_last)              # weights as the convolutions read them: no copies a call
 
     def forward(self, x, p_valid):
         if self.norm == 'group':

@@ -156,8 +156,12 @@ def test_group_normalised_networks():
     assert not any(isinstance(k, torch.nn.BatchNorm2d) for k in m.modules()) and not list(m.buffers())
     assert AlphaZeroC4(1, 12, norm='group')._tower[0]._gn2.num_groups == 1
     assert AlphaZeroC4(1, 12, norm='group', norm_groups=3)._tower[0]._gn2.num_groups == 3
+    assert m._tower[0]._c1.weight.is_contiguous(memory_format=torch.channels_last)
+    again = AlphaZeroC4(3, 32, norm='group').to(memory_format=torch.contiguous_format)
+    again.load_state_dict(m.state_dict())
     x = (torch.rand(5, 2, 6, 7) < 0.2).float()
     valid = torch.ones(5, 7, dtype=torch.bool)
+    assert torch.allclose(again(x, valid)[0], m(x, valid)[0], atol=1e-5)
     m.train()
     p, v = m(x, valid)
     m.eval()
