@@ -288,13 +288,14 @@ template <bool SILU> __device__ __forceinline__ float gn_act(float z, float low)
 
 // x - mean keeps its precision where the mean is large against the spread, with the mean as two floats mh + ml:
 // xhat = (x - mh) * rs - ml * rs
-struct GnNorm { double mean, rstd; float mh, rs, off; };
+struct GnNorm { double mean, rstd; float mh, rs, off, slack; };
 
 __device__ __forceinline__ GnNorm gn_norm(double mean, double rstd) {
     GnNorm k;
     k.mean = mean; k.rstd = rstd;
     k.mh = (float)mean; k.rs = (float)rstd;
     k.off = -(float)(mean - (double)k.mh) * k.rs;
+    k.slack = 0.0f;
     return k;
 }
 __device__ __forceinline__ float gn_xhat(const GnNorm& k, float x) { return fmaf(x - k.mh, k.rs, k.off); }
@@ -305,8 +306,17 @@ __device__ __forceinline__ void gn_affine(const GnNorm& k, float (&w)[VW], float
     for (int i = 0; i < VW; ++i) { b[i] = fmaf(k.off, w[i], b[i]); w[i] *= k.rs; }
 }
 
-__device__ __forceinline__ GnNorm gn_saved(const GnArgs& a, long n, int g) {
-    return gn_norm(a.stats[(n * a.G + g) * 2], a.stats[(n * a.G + g) * 2 + 1]);
+// (wmax: the largest |weight| of the thread's channels)
+__device__ __forceinline__ GnNorm gn_saved(const GnArgs& a, long n, int g, float wmax) {
+    GnNorm k = gn_norm(a.stats[(n * a.G + g) * 2], a.stats[(n * a.G + g) * 2 + 1]);
+    k.slack = fabsf(k.off) * wmax * a.near;
+    return k;
+}
+template <int VW> __device__ __forceinline__ float gn_largest(const float (&w)[VW]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) m = fmaxf(m, fabsf(w[i]));
+    return m;
 }
 
 #define GN_ROWS(VW) ((VW) == 8 ? 2 : 4)          // rows whose loads are on their way together
@@ -351,9 +361,9 @@ k_gn_apply(GnArgs a) {
     }
 }
 
-// dz of one value.  relu: z in 32 bits is off by less than 8 * 2^-24 * (|xhat w| + |b|) (three roundings of xhat, one
-// each of the product and the two sums, and |res| <= |xhat w| + |b| where z is small); closer to zero than twice that
-// `near` is set, and gn_relu_exact says.
+// dz of one value.  relu: z in 32 bits is off by less than 8 * 2^-24 * (|xhat w| + |b| + |off w|) (three roundings of xhat
+// and of its part off, one each of the product and the two sums, and |res| <= |xhat w| + |b| where z is small); closer to
+// zero than twice that `near` is set, and gn_relu_exact says.
 template <bool SILU>
 __device__ __forceinline__ float gn_dz(const GnArgs& a, const GnNorm& k, float x, float w, float b, float res, float dy, bool& near) {
     const float t = gn_xhat(k, x) * w, z = t + b + res;
@@ -361,7 +371,7 @@ __device__ __forceinline__ float gn_dz(const GnArgs& a, const GnNorm& k, float x
         const float sig = gn_sigmoid(z);
         return dy * (sig * fmaf(z, 1.0f - sig, 1.0f));
     }
-    near |= fabsf(z) < (fabsf(t) + fabsf(b)) * a.near;
+    near |= fabsf(z) < fmaf(fabsf(t) + fabsf(b), a.near, k.slack);
     return z <= a.low ? 0.0f : dy;
 }
 
@@ -399,10 +409,10 @@ k_gn_bwd_sums(GnArgs a) {
     double sa = 0.0, sx = 0.0;
     float dw[VW] = {}, db[VW] = {};
     if (p.on) {
-        const GnNorm k = gn_saved(a, p.n, p.g);
         float w[VW], b[VW];
         gn_param<VW>(a.w, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 1.0f, w);
         gn_param<VW>(a.b, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 0.0f, b);
+        const GnNorm k = gn_saved(a, p.n, p.g, gn_largest<VW>(w));
         constexpr int U = GN_ROWS(VW);
         uint32_t at = p.lane;
         for (int r0 = p.row; r0 < p.rows; r0 += U * a.rstep, at += U * p.step) {
@@ -458,10 +468,10 @@ k_gn_bwd_apply(GnArgs a) {
     gn_get_parts(a, p, sa, sx, lds);
     if (!p.on) return;
     const float ma = (float)(sa * a.inv), mx = (float)(sx * a.inv);
-    const GnNorm k = gn_saved(a, p.n, p.g);
     float w[VW], b[VW];
     gn_param<VW>(a.w, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 1.0f, w);
     gn_param<VW>(a.b, a.wtype, a.wide, p.g * a.Cg + p.col * VW, 0.0f, b);
+    const GnNorm k = gn_saved(a, p.n, p.g, gn_largest<VW>(w));
     // what the first pass wrote as the residual's gradient is dz, except where silu's was rounded to 16 bits
     const bool have = a.dres && (!SILU || sizeof(T) == 4);
     constexpr int U = GN_ROWS(VW);
@@ -516,8 +526,9 @@ k_gn_dparams(const float* __restrict__ dpart, long parts, int C, int wtype, void
 
 // ---- samples held in registers -----------------------------------------------------------------------------------
 // One pass over x (and dy, res): a team -- a wave, or a workgroup where a wave's registers do not hold a sample's slice --
-// loads its slice (some groups of a sample, 128 bytes of each row at least, or of several small samples), K vectors to a
-// thread, and has everything else in registers: 8 (12) bytes of traffic a value instead of 12 (16) in two passes.
+// loads its slice (some groups of a sample, 256 bytes of each row where it can, or of several small samples), K vectors to a
+// thread, and has everything else in registers: in float32, without a residual, 8 bytes of traffic a value instead of the
+// two passes' 12, and backward 12 instead of 20.
 // A thread holds VW neighbouring channels of one group in each of its rows.  The bits of its index in the team are, from
 // the lowest: column within the group (cb), group within the slice (gb), row (rb), sample (sb).  Sums over a group are
 // butterflies over the column and row bits, so a wave's loads run along memory whatever the group's width.
@@ -626,6 +637,7 @@ k_gn_bwd_held(GnArgs a) {
     gn_param<VW>(a.b, a.wtype, a.wide, seated ? c : 0, 0.0f, b);
 #pragma unroll
     for (int i = 0; i < VW; ++i) dw[i] = db[i] = 0.0f;
+    const float wmax = gn_largest<VW>(w);
     const long step = ((long)a.C << a.rb) * (long)sizeof(T);
     const uint32_t lane = (uint32_t)(((p.sample * a.HW + p.row) * a.C + c) * (int)sizeof(T));
     for (long batch = walker; batch < batches; batch += a.walkers) {
@@ -642,7 +654,7 @@ k_gn_bwd_held(GnArgs a) {
             if (a.res) r[k] = in ? gn_raw<T, VW>(a.res, base + k * step, lane) : V{};
         }
         GnNorm s = {};
-        if (on) s = gn_saved(a, n, g);
+        if (on) s = gn_saved(a, n, g, wmax);
         float dz[SILU ? K : 1][VW], fa = 0.0f, fx = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -987,6 +999,7 @@ int az_group_norm_act(const az_group_norm* g, const void* x, const void* weight,
     if (!x || !y) return az_fail("az_group_norm_act: null pointer");
     const int64_t need = az_group_norm_workspace_bytes(g, 0);
     if (workspace_bytes < need || (need && !workspace)) return az_fail("az_group_norm_act: workspace too small");
+    if ((uintptr_t)workspace % 16) return az_fail("az_group_norm_act: workspace is aligned to 16 bytes");
     const void* all[] = {x, y, residual};
     const int VW = gn_width(g, all, 3);
     GnArgs a = gn_base(g, VW);
@@ -1010,6 +1023,7 @@ int az_group_norm_act_backward(const az_group_norm* g, const void* dy, const voi
     const int64_t need = az_group_norm_workspace_bytes(g, 1);
     if (workspace_bytes < need || (need && !workspace))
         return az_fail("az_group_norm_act_backward: workspace too small");
+    if ((uintptr_t)workspace % 16) return az_fail("az_group_norm_act_backward: workspace is aligned to 16 bytes");
     const void* all[] = {dy, x, residual, dx, dresidual};
     const int VW = gn_width(g, all, 5);
     GnArgs a = gn_base(g, VW);

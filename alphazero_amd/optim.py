@@ -296,7 +296,7 @@ class FlatAdamW(torch.optim.Optimizer):
         steps = float(self.steps)
         packed['state'] = {}
         for p, at in self._places:
-            s = dict(step=torch.tensor(steps), exp_avg=self._cut(m, p, at).clone(), exp_avg_sq=self._cut(v, p, at).clone())
+            s = dict(step=torch.tensor(steps, dtype=torch.float64), exp_avg=self._cut(m, p, at).clone(), exp_avg_sq=self._cut(v, p, at).clone())
             if p.dtype == torch.bfloat16:
                 s['master'] = self._cut(self.flat_p, p, at).clone()
             packed['state'][number[id(p)]] = s

@@ -455,6 +455,31 @@ def test_channels_last_weights_keep_their_layout():
     assert torch.allclose(conv.weight, ref, rtol=1e-6, atol=1e-7)
 
 
+@pytest.mark.parametrize('bits', [8, 32])
+def test_more_elements_than_32_bits_count(bits):
+    """2^31 + 300 elements: the first and last ones against the formula, a second tensor behind them."""
+    from alphazero_amd.optim import FlatAdamW
+    n = 2 ** 31 + 300
+    p = [torch.nn.Parameter(torch.zeros(n, device='cuda')), torch.nn.Parameter(torch.full((3,), 2.0, device='cuda'))]
+    with torch.no_grad():
+        p[0][-300:] = 1.0
+    opt = FlatAdamW(p, lr=1e-2, weight_decay=0.1, state_bits=bits)
+    assert opt._places[1][1] > 2 ** 31
+    p[0].grad[-300:] = torch.linspace(-1, 1, 300, device='cuda')
+    p[1].grad.fill_(-3.0)
+    opt.step()
+    g = torch.linspace(-1, 1, 300, device='cuda').double()
+    want = 1 - 1e-3 - 1e-2 * g / (g.abs() + 1e-8)
+    assert bool(((p[0][-300:].double() - want).abs() <= 20 * U).all()) and not p[0][:1000].any()
+    assert bool(((p[1].double() - (2 * (1 - 1e-3) + 1e-2)).abs() <= 24 * U).all())
+    m, _ = opt.state_values()
+    at = opt._places[1][1]
+    assert bool(((m[at:at + 3] + 0.3).abs() <= (0.3 * 2 ** -3 if bits == 8 else 1e-7)).all())
+    del m
+    opt.step()
+    assert opt.steps == 2
+
+
 def test_another_stream():
     from alphazero_amd.optim import FlatAdamW
     a, b = (_params(SIZES, 13) for _ in range(2))

@@ -169,6 +169,18 @@ def test_relu_cuts_the_gradient_where_the_sum_passes_zero_in_64_bits():
     assert torch.equal(got['dr'].double()[sure], want['dr'][sure]) and float(sure.double().mean()) > 0.999
 
 
+def test_relu_cuts_exactly_in_groups_far_from_zero():
+    """Means a thousand spreads away, no bias, no residual: z passes zero where x passes the mean, which lies between two
+    float32 values of x."""
+    n, c, groups, h, w = 64, 32, 4, 8, 8
+    x, wt, _, _, _ = _inputs(n, c, h, w, torch.float32, torch.float32, False, 18, 1000.0, 1e-3)
+    b, dy = torch.zeros(c, device='cuda'), torch.ones_like(x)
+    want, _ = _reference(x, groups, wt, b, None, dy, 'relu')
+    got = _run(x, groups, wt, b, None, dy, 'relu')
+    # db counts the open values; the 64-bit mean itself is good to 1e-13 of values 1e-4 apart, so no count may differ
+    assert torch.equal(got['db'].double(), want['db'])
+
+
 def test_constant_groups_have_their_bias():
     """Groups of equal values (an empty board behind a convolution): variance 0, z = bias exactly, relu open where
     bias > 0 and shut where it is 0 or below, no gradient through x."""

@@ -100,9 +100,11 @@ def test_c_entries_refuse_null_pointers_and_small_workspaces():
     assert b'null' in lib.az_last_error()
     assert lib.az_group_norm_act_backward(C.byref(g), p, p, None, None, None, p, p, None, None, p, p, 1 << 40, None) != 0
     assert b'without a residual' in lib.az_last_error()
-    if need:
-        assert lib.az_group_norm_act_backward(C.byref(g), p, p, None, None, None, p, p, p, p, None, p, need - 1, None) != 0
-        assert b'workspace' in lib.az_last_error()
+    assert need > 0
+    assert lib.az_group_norm_act_backward(C.byref(g), p, p, None, None, None, p, p, p, p, None, p, need - 1, None) != 0
+    assert b'workspace' in lib.az_last_error()
+    assert lib.az_group_norm_act_backward(C.byref(g), p, p, None, None, None, p, p, p, p, None, C.c_void_p(264), need, None) != 0
+    assert b'aligned' in lib.az_last_error()
     assert lib.az_group_norm_workspace_bytes(None, 0) == -1
 
 
