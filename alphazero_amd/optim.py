@@ -185,13 +185,14 @@ class FlatAdamW(torch.optim.Optimizer):
                 p.grad = grad
                 self._grads.append(grad)
         self._addresses = [p.data_ptr() for p, _ in self._places]
+        self._still = _lib.autograd().Places([p for p, _ in self._places], self._grads)
         b = _lib.AdamWBuffers()
         for name, t in (('p', self.flat_p), ('g', self.flat_g), ('p16', self.flat_p16), ('g16', self.flat_g16), ('m', self.flat_m),
                         ('v', self.flat_v), ('m8', self.codes_m), ('v8', self.codes_v), ('top', self.tops),
                         ('step', self._step_dev)):
             setattr(b, name, None if t is None else t.data_ptr())
         self._buffers = b
-        self._args = (_lib.AdamWRun * len(self._runs))()
+        self._args, self._settings = (_lib.AdamWRun * len(self._runs))(), None
         for a, (k, is16, first) in zip(self._args, self._runs):
             a.first_block, a.half, a.lr_index = first, int(is16), k
         self._bound = True
@@ -229,6 +230,8 @@ class FlatAdamW(torch.optim.Optimizer):
                 p.grad = grad
 
     def _rebind(self):
+        if self._still.in_place():
+            return
         if [p.data_ptr() for p, _ in self._places] != self._addresses:
             raise _lib.AzError('a parameter of FlatAdamW was moved out of the flat buffer (module.to(), p.data = ...): move the '
                                'module first, then construct the optimizer')
@@ -242,9 +245,11 @@ class FlatAdamW(torch.optim.Optimizer):
                 p.grad = grad
 
     def _launch(self, lr_dev, guard, guard_limit):
-        for a, (k, _, _) in zip(self._args, self._runs):
+        settings = [(g['lr'], g['betas'], g['eps'], g['weight_decay']) for g in self.param_groups]
+        for a, (k, _, _) in zip(self._args, self._runs) if settings != self._settings else ():
             g = self.param_groups[k]
             a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = float(g['lr']), g['betas'], g['eps'], g['weight_decay']
+        self._settings = settings
         _lib.launch(self.device, self.lib.az_adamw_step, self._buffers, self._blocks, self._args, len(self._runs), self.state_bits,
                     _lib.ptr(lr_dev), self.seed, _lib.ptr(guard), guard_limit, self.withheld.data_ptr())
 

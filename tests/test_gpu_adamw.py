@@ -534,29 +534,53 @@ class _Writer:
         self.rows.append((tag, float(value), int(step)))
 
 
-@pytest.mark.parametrize('norm,bits', [('group', 32), ('group', 8), ('batch', 8)])
-def test_training_worker_with_group_norm_and_adamw(norm, bits):
-    """Ten steps of TrainingWorker, eager and recorded from the fourth on: the same batches; losses, weights and the step
-    count agree.  (8 bits: a rounding that falls the other way because a convolution's gradient differs in its last
-    bits moves a moment by a step, 12 % of one element's update of at most 3 lr.)"""
+@pytest.mark.parametrize('norm,bits,record', [('group', 32, True), ('group', 8, True), ('group', 8, False), ('batch', 8, True)])
+def test_training_worker_with_group_norm_and_adamw(norm, bits, record):
+    """Ten steps of TrainingWorker, three eager and the rest replayed (or all eager), each checked from its own start: the
+    logged losses against the network with the weights before the step on the same batch, the gradients against autograd
+    there, and the update against an optimizer of the same state that steps eagerly on the same gradients: the same bits.
+    (Two trainings are not compared: the library's convolutions add in no fixed order, and Adam turns the last bits of
+    a gradient next to zero into a step of the full rate.)  A loss is a mean of values below 5 whose logits went through
+    7 layers of sums of up to 288 terms, each off by at most 288 u of its magnitudes: 7 * 288 * u * 5 < 1e-3; a gradient
+    passes twice as many and is a sum over 32 boards of 42 cells: 1e-2 of its norm."""
+    import copy
+    from alphazero_amd.loss import masked_cross_entropy
     from alphazero_amd.optim import FlatAdamW
     from alphazero_amd.training import TrainingWorker
     dev = torch.device('cuda:0')
-    window, runs = _window(dev), []
-    for record in (False, True):
-        torch.manual_seed(11)
-        writer = _Writer()
-        tw = TrainingWorker(_job(norm, bits), _Server(), window, writer, dev, record_step=record)
-        assert isinstance(tw._optimizer, FlatAdamW) and (tw._hand is not None) == (norm == 'batch')
-        assert [tw.process_batch() for _ in range(10)] == list(range(1, 11))
-        assert (tw._graph is not None) == record and tw._optimizer.steps == 10
-        runs.append((writer.rows, [p.detach().clone() for p in tw.model.parameters()]))
-    (rows_a, pa), (rows_b, pb) = runs
-    assert [(r[0], r[2]) for r in rows_a] == [(r[0], r[2]) for r in rows_b]
-    for ra, rb in zip(rows_a, rows_b):
-        assert np.isfinite(ra[1]) and abs(ra[1] - rb[1]) <= (1e-3 if bits == 8 else 1e-4) * max(1.0, abs(ra[1])), (ra, rb)
-    for a, b in zip(pa, pb):
-        assert (a - b).abs().max() <= 10 * 3 * 1e-3 * (0.125 if bits == 8 else 0.01)
+    window = _window(dev)
+    torch.manual_seed(11)
+    writer = _Writer()
+    tw = TrainingWorker(_job(norm, bits), _Server(), window, writer, dev, record_step=record)
+    opt = tw._optimizer
+    assert isinstance(opt, FlatAdamW) and (tw._hand is not None) == (norm == 'batch')
+    taken, batch = [], tw._batch
+    tw._batch = lambda: taken.append(batch()) or taken[-1]
+    for k in range(10):
+        before = copy.deepcopy(tw.model.state_dict())
+        state = opt.state_dict()
+        writer.rows.clear()
+        assert tw.process_batch() == k + 1
+        recorded = record and k >= tw.EAGER_STEPS
+        x, p, z, valid = (tw._gx, tw._gp, tw._gz, tw._gvalid) if recorded else taken[-1][:4]
+        shadow = tw._config.Model().to(dev)
+        shadow.load_state_dict(before)
+        shadow.train()
+        other = FlatAdamW(shadow.parameters(), state_bits=bits)
+        logits, v = shadow(x, valid.bool())
+        policy, value = masked_cross_entropy(logits, p, valid.bool()).mean(), ((z.reshape(-1, 1) - v) ** 2).mean()
+        (policy + value).backward()
+        logged = {r[0]: r[1] for r in writer.rows}
+        assert abs(logged['loss/policy'] - policy.item()) < 1e-3 and abs(logged['loss/value'] - value.item()) < 1e-3, k
+        for (name, a), b in zip(tw.model.named_parameters(), shadow.parameters()):
+            if norm == 'batch' and name == '_policy_head._cbr.0.bias':
+                continue                                           # (zero but for rounding: batch-norm takes the bias out)
+            assert (a.grad - b.grad).norm() <= 1e-2 * b.grad.norm() + 1e-6, (k, name)
+        other.load_state_dict(state)
+        other.flat_g.copy_(opt.flat_g)
+        other.step()
+        assert torch.equal(other.flat_p, opt.flat_p) and all(torch.equal(a, b) for a, b in zip(other.state_values(), opt.state_values())), k
+    assert (tw._graph is not None) == record and opt.steps == 10 and abs(opt.param_groups[0]['lr'] - 1e-4) < 1e-12
 
 
 def test_a_writer_may_keep_what_it_is_given():
