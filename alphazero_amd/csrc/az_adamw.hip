@@ -26,12 +26,14 @@
 #include "../../include/azhip.h"
 #include "az_host.h"
 
-#define ADAMW_BLOCK 256          // elements: four of each lane of a wave
+#define ADAMW_BLOCK AZ_ADAMW_BLOCK   // elements: four of each lane of a wave
+static_assert(ADAMW_BLOCK == 4 * 64, "a wave takes a block");
 // A wave takes a block, four neighbouring elements to a lane, so that every load and store of a wave is one piece of memory.
-// Bound by memory in 32 bits (28 bytes an element): 46 M parameters 222 us = 5.8 TB/s, where a copy of as much has 4.7 to 5.2.
-// In 8 bits (16 bytes) by memory and instructions alike: 129 us = 5.7 TB/s, and some 110 instructions an element, a quarter
-// of them the random numbers.  Workgroups of 512 threads that take one block a wave and end: their traffic moves along memory as
-// one front.  2048 workgroups that walk over the blocks: 238 to 250 and 137 to 146 us.
+// Bound by memory in 32 bits (28 bytes an element): 46 M parameters 222 us = 5.8 TB/s, where a copy of as much has 4.7 to
+// 5.2.  In 8 bits (16 bytes) by memory and instructions alike: 129 us = 5.7 TB/s, and 77 vector instructions an element
+// keep the SIMDs busy for 69 % of it, the random numbers about a sixth of them.  Workgroups of 512 threads that take one
+// block a wave and end: their traffic moves along memory as one front.  2048 workgroups that walk over the blocks: 238 to
+// 250 and 137 to 146 us.
 #define ADAMW_THREADS 512
 #define ADAMW_GOLDEN 0x9E3779B97F4A7C15ull
 

@@ -458,8 +458,9 @@ int  az_sgd_momentum_guarded(float* params, const float* grads, float* momentum_
  *   z = (x - mean) * rstd * weight[c] + bias[c] (+ residual),  y = act(z),
  * mean and rstd = 1 / sqrt(var + eps) over the cells and the channels / groups channels of a sample's group; sums and
  * statistics in 64 bits, the rest in 32, one rounding to the tensors' type.  relu and its gradient pass a NaN on.
- * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any size and alignment
- * (16-byte aligned tensors and groups of a multiple of 4 channels, 8 in 16 bits, run fastest).                    */
+ * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any size (a sample of at most
+ * 2^31 - 1 values, 2^28 channels) and alignment (16-byte aligned tensors and groups of a multiple of 4 channels, 8 in 16
+ * bits, run fastest).                                                                                              */
 #define AZ_F32  0
 #define AZ_BF16 1
 #define AZ_F16  2
