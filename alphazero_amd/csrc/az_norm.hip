@@ -18,7 +18,7 @@
 //   4096 x 42 x 128, bfloat16, with residual and relu     forward 28 us for 132 MB, backward 46 + 4 us for 220 MB    4.7, 4.4 TB/s
 //   128 x 42 x 256, float32, as in a training step of the shipped batch         forward 6, backward 8 + 3 us
 //   1 x 42 x 256, float32, one position                                         3.8 us, a launch that does nothing 2.8
-//   61 x 361 x 192, float16, silu     forward 10, backward 18 + 4 us: bound by instructions and the one wave of workgroups
+//   61 x 361 x 192, float16, silu     forward 10, backward 15 + 4 us: bound by instructions and the one wave of workgroups
 //   3 x 4096 x 320, bfloat16, silu    5.7 + 7.5 us: two launches, x from the caches the second time
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -816,6 +816,8 @@ static void gn_plan_split(GnArgs& a, int VW, int dtype) {
 //   Slices take 256 bytes of a row, less only where no team holds that: 42 cells x 128 channels, backward, 4096 boards in
 // bfloat16: 54 us at 256 bytes (a workgroup, K = 3), 61 at 128 (a wave, K = 6), 67 at 64.  Slices of 64 bytes share lines;
 // with neighbours on one die they still beat the two passes (64 x 1024 cells x 128 channels, forward: 12.5 against 16.9 us).
+//   Workgroups of 1024 do not go deeper than this table: 3 x 4096 cells x 320 channels, bfloat16, forward, takes 24 us held
+// 32 vectors of 4 bytes deep and 12.4 in two passes; 64 x 1024 cells, 16 deep, 66 and 53.
 //   A wave is taken before a workgroup: it needs no barrier (hw 1, 8192 x 512 channels: 7 against 14 us forward).
 static bool gn_plan_held(GnArgs& a, int VW, int dtype, bool silu, bool backward, int& K, int& threads) {
     // vectors of a thread that its registers hold, in a team of a wave, 256 and 1024 threads: forward, backward, with silu
@@ -854,13 +856,19 @@ static bool gn_plan_held(GnArgs& a, int VW, int dtype, bool silu, bool backward,
             threads = kind == 2 ? 1024 : 256;
             if (backward) {
                 const long batches = (a.N + (1 << a.sb) - 1) >> a.sb, teams = kind == 0 ? 4 : 1;
-                // Workgroups: enough for 64 KiB on their way to each compute unit (8192 boards x 128 channels, float32: 512
-                // take 171 us, 1024 178; at 30 channels in 5 groups, half the lanes idle, 512 take 19.8 and 1024 17.0), but
-                // no more than a sixteenth of the traffic in partial sums (8192 x 512 channels of one cell: 512 take
-                // 14.4 us, 2048 24.5)
+                // Workgroups to each compute unit: enough for 64 KiB on their way (8192 boards x 128 channels, float32: 512
+                // take 171 us, 1024 178; at 30 channels in 5 groups, half the lanes idle, 512 take 19.8 and 1024 17.0);
+                // two of 256 threads, one of which works while the other's loads are on their way (81 cells x 128
+                // channels, 4096 boards, bfloat16: 144 us with one, 106 with two, 118 with three); one of 1024, which
+                // fills the registers (61 x 361 cells x 192 channels, float16, silu: 18.7 us with two, 16.7 with one).
+                // But no more than a sixteenth of the traffic in partial sums (8192 x 512 channels of one cell: 512 take
+                // 14.4 us, 2048 24.5).
                 const long lanes = (long)threads * a.cpg / (1 << cb) * (a.G < (1 << gb) ? a.G : 1 << gb) / (1 << gb);
                 const long flight = 3 * lanes * K * VW * gn_size(dtype);
-                long blocks = 256 * (65536 / (flight > 0 ? flight : 1) + 1) / slices;
+                long per = 65536 / (flight > 0 ? flight : 1) + 1;
+                if (threads == 1024) per = 1;
+                else if (per < 2) per = 2;
+                long blocks = 256 * per / slices;
                 const long most_rows = a.N * a.HW * gn_size(dtype) * 3 / 128;
                 if (blocks > 1536 / slices) blocks = 1536 / slices;
                 if (blocks > most_rows) blocks = most_rows;
