@@ -1,7 +1,8 @@
-// az_torch.cpp -- autograd functions over the C ABI, and what else is asked of tensors at every step, for calls whose launches are shorter than Python's way to them: a
-// step of the group norm at the shipped batch of 128 is 16 us on the device; its autograd function written in Python took 73 to
-// 113 us a call on the host, this one 42 to 70 (of which the engine's own threads are 30).  Host code only; the entry
-// points of libazhip.so are handed over as addresses (alphazero_amd/_lib.py), so that both sides use one library.
+// az_torch.cpp -- autograd functions over the C ABI, and what else is asked of tensors at every step, for calls whose launches
+// are shorter than Python's way to them: a step of the group norm at the shipped batch of 128 is 18 us on the device; its
+// autograd function written in Python took 73 to 115 us a call on the host, this one 42 to 70 (of which the engine's own
+// threads are 30).  Host code only; the entry points of libazhip.so are handed over as addresses (alphazero_amd/_lib.py), so
+// that both sides use one library.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <c10/hip/HIPStream.h>

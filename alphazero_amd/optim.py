@@ -136,6 +136,8 @@ class FlatAdamW(torch.optim.Optimizer):
                 order += [(k, half, p) for p in g['params'] if p.requires_grad and (p.dtype == torch.bfloat16) == half]
         if not order:
             raise ValueError('no parameter requires a gradient')
+        if len({id(p) for _, _, p in order}) < len(order):
+            raise ValueError('a parameter is given twice')
         dev = order[0][2].device
         if dev.type != 'cuda':
             raise _lib.AzError('FlatAdamW runs on the GPU (az_adamw_step); use torch.optim.AdamW for CPU tensors')
@@ -245,10 +247,10 @@ class FlatAdamW(torch.optim.Optimizer):
                 p.grad = grad
 
     def _launch(self, lr_dev, guard, guard_limit):
-        settings = [(g['lr'], g['betas'], g['eps'], g['weight_decay']) for g in self.param_groups]
+        # (as numbers: a rate in a tensor, betas in a list may be changed in place)
+        settings = [(float(g['lr']), *map(float, g['betas']), float(g['eps']), float(g['weight_decay'])) for g in self.param_groups]
         for a, (k, _, _) in zip(self._args, self._runs) if settings != self._settings else ():
-            g = self.param_groups[k]
-            a.lr, (a.beta1, a.beta2), a.eps, a.weight_decay = float(g['lr']), g['betas'], g['eps'], g['weight_decay']
+            a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = settings[k]
         self._settings = settings
         _lib.launch(self.device, self.lib.az_adamw_step, self._buffers, self._blocks, self._args, len(self._runs), self.state_bits,
                     _lib.ptr(lr_dev), self.seed, _lib.ptr(guard), guard_limit, self.withheld.data_ptr())

@@ -440,6 +440,26 @@ def test_a_frozen_parameter_stays_and_a_closure_is_called():
     assert float(opt.step(closure)) < float(first) and torch.equal(p[1], frozen) and 1 not in opt.state_dict()['state']
 
 
+def test_settings_that_change_in_place():
+    """A rate held in a tensor, as torch's schedulers fill it, and betas held in a list."""
+    from alphazero_amd.optim import FlatAdamW
+    a, b = (_params(SIZES, 21) for _ in range(2))
+    rate, betas = torch.tensor(1e-2), [0.9, 0.999]
+    oa, ob = FlatAdamW(a, lr=rate, betas=betas), FlatAdamW(b, lr=float(rate))
+    for k in range(4):
+        for q in (a, b):
+            for p, g in zip(q, _grads(q, 30 + k)):
+                p.grad.copy_(g)
+        oa.step()
+        ob.step()
+        assert torch.equal(oa.flat_p, ob.flat_p), k
+        rate.mul_(0.5)
+        ob.param_groups[0]['lr'] = float(rate)
+        if k == 1:
+            betas[0] = 0.8
+            ob.param_groups[0]['betas'] = (0.8, 0.999)
+
+
 def test_channels_last_weights_keep_their_layout():
     from alphazero_amd.optim import FlatAdamW
     conv = torch.nn.Conv2d(8, 16, 3).cuda().to(memory_format=torch.channels_last)

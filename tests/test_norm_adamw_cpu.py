@@ -148,6 +148,14 @@ def test_flat_adamw_refuses_what_it_cannot_do():
         FlatAdamW([torch.nn.Parameter(torch.zeros(3), requires_grad=False)])
 
 
+@pytest.mark.filterwarnings('ignore:optimizer contains a parameter group with duplicate')
+def test_adamw_refuses_a_parameter_twice():
+    from alphazero_amd.optim import FlatAdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    with pytest.raises(ValueError, match='given twice'):
+        FlatAdamW([p, torch.nn.Parameter(torch.ones(2)), p])
+
+
 def test_group_normalised_networks():
     from alphazero_amd.models import AlphaZero, AlphaZeroC4, GroupNormBlock
     from alphazero_amd.net import TTTNetF32, pack_c4_blob_f32, pack_ttt_blob_f32
