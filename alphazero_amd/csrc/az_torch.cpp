@@ -38,6 +38,13 @@ int32_t type_of(const Tensor& t) {
 // channels last, without a copy where it is that already
 Tensor last(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.contiguous(at::MemoryFormat::ChannelsLast); }
 
+// `t` is what a kernel that goes by `like` takes it for
+void same(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == like.device(),
+                "group_norm_act: a saved tensor came back as another one (", t.scalar_type(), t.sizes(), " on ", t.device(), "; it was ",
+                type, sizes, " on ", like.device(), ")");
+}
+
 az_group_norm descriptor(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups, double eps, int64_t act) {
     const int64_t cells = x.dim() == 4 ? x.size(2) * x.size(3) : 1;
     TORCH_CHECK_VALUE(x.size(0) <= INT32_MAX && cells <= INT32_MAX && x.size(1) <= INT32_MAX, "tensor too large");
@@ -84,17 +91,28 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 
     static variable_list backward(AutogradContext* ctx, variable_list dys) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &residual = saved[3], &stats = saved[4];
+        const Tensor &stats_ = saved[4], &dy_ = dys[0];
+        const int64_t groups = ctx->saved_data["groups"].toInt();
         const int64_t needs = ctx->saved_data["needs"].toInt();
         variable_list grads(7);
         {
             const at::AutoGradMode off(false);
-            const az_group_norm g = descriptor(x, weight, bias, ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(),
-                                               ctx->saved_data["act"].toInt());
-            const c10::DeviceGuard guard(x.device());
-            const Tensor dy = last(dys[0]);
+            const c10::DeviceGuard guard(dy_.device());
+            // a saved-tensor hook may have given the values back in another order of memory, or other tensors altogether
+            const Tensor &x_ = saved[0], &w_ = saved[1], &b_ = saved[2], &r_ = saved[3];
+            const int64_t channels = dy_.size(1);
+            same(x_, dy_, dy_.sizes(), dy_.scalar_type());
+            if (r_.defined()) same(r_, dy_, dy_.sizes(), dy_.scalar_type());
+            for (const Tensor& t : {w_, b_})
+                if (t.defined()) same(t, dy_, {channels}, t.scalar_type() == at::kFloat ? at::kFloat : dy_.scalar_type());
+            TORCH_CHECK(!w_.defined() || !b_.defined() || w_.scalar_type() == b_.scalar_type(), "group_norm_act: weight and bias of two types were saved");
+            same(stats_, dy_, {dy_.size(0), groups, 2}, at::kDouble);
+            const Tensor x = last(x_), residual = r_.defined() ? last(r_) : r_, weight = w_.defined() ? w_.contiguous() : w_,
+                         bias = b_.defined() ? b_.contiguous() : b_, stats = stats_.contiguous(), dy = last(dy_);
+            const az_group_norm g = descriptor(x, weight, bias, groups, ctx->saved_data["eps"].toDouble(), ctx->saved_data["act"].toInt());
+            const Tensor* inputs[] = {&x, &weight, &bias, &residual};
             for (int i = 0; i < 4; ++i)
-                if (needs >> i & 1) grads[i] = at::empty_like(saved[i]);
+                if (needs >> i & 1) grads[i] = at::empty_like(*inputs[i]);
             int64_t bytes;
             const Tensor ws = workspace(g, 1, x, bytes);
             check(az.group_norm_act_backward(&g, ptr(dy), ptr(x), ptr(weight), ptr(bias), ptr(residual), (const double*)ptr(stats),
