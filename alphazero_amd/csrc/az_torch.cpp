@@ -38,6 +38,13 @@ int32_t type_of(const Tensor& t) {
 // channels last, without a copy where it is that already
 Tensor last(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.contiguous(at::MemoryFormat::ChannelsLast); }
 
+// The kernels read memory only; what else a tensor can carry must not be lost without a word.
+void plain(const Tensor& t) {
+    if (!t.defined()) return;
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "group_norm_act has no forward-mode derivative on the GPU");
+    TORCH_CHECK_NOT_IMPLEMENTED(t.has_storage(), "group_norm_act takes tensors with memory of their own on the GPU: no vmap, no functorch transforms");
+}
+
 // `t` is what a kernel that goes by `like` takes it for
 void same(const Tensor& t, const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
     TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == like.device(),
@@ -96,6 +103,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         const int64_t needs = ctx->saved_data["needs"].toInt();
         variable_list grads(7);
         {
+            plain(dy_);
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy_.device());
             // a saved-tensor hook may have given the values back in another order of memory, or other tensors altogether
@@ -132,6 +140,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                       const std::optional<Tensor>& residual, int64_t groups, double eps, int64_t act) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    for (const Tensor& t : {x, w, b, r}) plain(t);
     const bool grad = at::GradMode::is_enabled() &&
                       (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()) || (r.defined() && r.requires_grad()));
     if (grad) return GroupNormAct::apply(x, weight, bias, residual, groups, eps, act);

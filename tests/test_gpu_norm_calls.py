@@ -49,3 +49,24 @@ def test_saved_tensors_that_come_back_as_others_are_refused(other):
     x, wt, b, r, dy = _inputs(6, 32, 6, 7, torch.float32, torch.float32, True, 32)
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other), pytest.raises(RuntimeError, match='came back as another one'):
         _grads(x, 4, wt, b, r, dy)
+
+
+def test_forward_mode_tangents_are_refused():
+    """In x, and in the gradient that comes into the backward pass; a batch of such gradients likewise.  Calls without them
+    go on as before."""
+    import torch.autograd.forward_ad as forward_ad
+    from alphazero_amd.norm import group_norm_act
+    x, wt, b, r, dy = _inputs(3, 16, 6, 7, torch.float32, torch.float32, True, 33)
+    want = _run(x, 4, wt, b, r, dy, 'relu')
+    with forward_ad.dual_level():
+        with torch.no_grad(), pytest.raises(NotImplementedError, match='forward-mode'):
+            group_norm_act(forward_ad.make_dual(x, torch.ones_like(x)), 4, wt, b, residual=r)
+        leaf = x.detach().requires_grad_()
+        y = group_norm_act(leaf, 4, wt, b, residual=r)
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            torch.autograd.grad(y, leaf, forward_ad.make_dual(dy, torch.ones_like(dy)))
+        y = group_norm_act(leaf, 4, wt, b, residual=r)
+        assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], want['dx'])
+    y = group_norm_act(leaf, 4, wt, b, residual=r)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.autograd.grad(y, leaf, torch.stack([dy, dy]), is_grads_batched=True)

@@ -1,0 +1,33 @@
+"""What the group norm's GPU entry refuses before it touches memory, asked with CPU tensors where no GPU is needed for it;
+and its kernels' limits, through C entries that launch nothing."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from alphazero_amd import _lib
+from alphazero_amd.norm import group_norm_act
+
+
+def _entry(x, w=None, b=None, r=None):
+    return _lib.autograd().group_norm_act(x, w, b, r, 2, 1e-5, 1)
+
+
+@pytest.mark.parametrize('which', ['x', 'w', 'b', 'r'])
+@pytest.mark.parametrize('grad', [False, True])
+def test_forward_mode_tangents_are_refused(which, grad):
+    """A dual tensor: its tangent would be lost in the kernel.  (The CPU statement has the derivative.)"""
+    t = dict(x=torch.randn(2, 4, 3, 3), w=torch.ones(4), b=torch.zeros(4), r=torch.randn(2, 4, 3, 3))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        t[which] = forward_ad.make_dual(t[which], torch.ones_like(t[which]))
+        with pytest.raises(NotImplementedError, match='forward-mode'):
+            _entry(**t)
+        y = group_norm_act(t['x'], 2, t['w'], t['b'], residual=t['r'])
+        assert forward_ad.unpack_dual(y).tangent is not None
+
+
+def test_functorch_transforms_are_refused():
+    x = torch.randn(2, 4, 3, 3)
+    for call in (lambda: torch.func.vmap(lambda t: _entry(t))(x[None]), lambda: torch.func.grad(lambda t: _entry(t).sum())(x),
+                 lambda: torch.func.jvp(_entry, (x,), (x,)), lambda: torch.func.vmap(lambda t: _entry(x, t))(torch.ones(3, 4))):
+        with pytest.raises(NotImplementedError, match='group_norm_act'):
+            call()
