@@ -5,6 +5,8 @@
 // that both sides use one library.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/azhip.h"
@@ -42,7 +44,16 @@ Tensor last(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.contiguo
 void plain(const Tensor& t) {
     if (!t.defined()) return;
     TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "group_norm_act has no forward-mode derivative on the GPU");
-    TORCH_CHECK_NOT_IMPLEMENTED(t.has_storage(), "group_norm_act takes tensors with memory of their own on the GPU: no vmap, no functorch transforms");
+    TORCH_CHECK_NOT_IMPLEMENTED(t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch(),
+                                "group_norm_act takes tensors with memory of their own on the GPU: no vmap, no functorch transforms");
+}
+
+// A launch goes past torch's dispatcher: a tracer would record the allocation of the result and nothing that fills it.
+void untraced() {
+    using c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
+                                    !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::FAKE),
+                                "group_norm_act cannot be traced on the GPU (torch.jit.trace, make_fx, torch.export, fake tensors)");
 }
 
 // `t` is what a kernel that goes by `like` takes it for
@@ -103,6 +114,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         const int64_t needs = ctx->saved_data["needs"].toInt();
         variable_list grads(7);
         {
+            untraced();
             plain(dy_);
             const at::AutoGradMode off(false);
             const c10::DeviceGuard guard(dy_.device());
@@ -140,6 +152,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 Tensor group_norm_act(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                       const std::optional<Tensor>& residual, int64_t groups, double eps, int64_t act) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    untraced();
     for (const Tensor& t : {x, w, b, r}) plain(t);
     const bool grad = at::GradMode::is_enabled() &&
                       (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()) || (r.defined() && r.requires_grad()));

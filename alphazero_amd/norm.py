@@ -47,8 +47,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act='relu', 
     x [N, C, H, W] (kept in torch.channels_last; other layouts are copied to it first) or [N, C], float32, bfloat16 or
     float16; residual of x's shape and type; weight and bias [C], both float32 or both of x's type; act 'none', 'relu'
     or 'silu'.  Returns a channels-last tensor of x's type.  Differentiable once with respect to x, weight, bias and
-    residual, on the GPU by a backward pass alone: tensors with a forward-mode tangent, torch.func's transforms and batches of
-    gradients are refused there.  Statistics are kept in 64 bits and the sign of a value next to zero, at which relu cuts the gradient, is
+    residual, on the GPU by a backward pass alone: tensors with a forward-mode tangent, torch.func's transforms, batches of
+    gradients and tracing (torch.jit.trace, make_fx, torch.export) are refused there.  Statistics are kept in 64 bits and the sign of a value next to zero, at which relu cuts the gradient, is
     decided in them; an empty group of values (H * W * C / num_groups == 1) has variance 0."""
     if act not in ACTS:
         raise ValueError(f"act is 'none', 'relu' or 'silu', got {act!r}")

@@ -70,3 +70,22 @@ def test_forward_mode_tangents_are_refused():
     y = group_norm_act(leaf, 4, wt, b, residual=r)
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.autograd.grad(y, leaf, torch.stack([dy, dy]), is_grads_batched=True)
+
+
+@pytest.mark.filterwarnings('ignore')
+def test_tracing_is_refused_and_leaves_nothing_behind():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from alphazero_amd.norm import GroupNormAct, group_norm_act
+    x, wt, b, r, dy = _inputs(3, 16, 6, 7, torch.float32, torch.float32, True, 34)
+    want = group_norm_act(x, 4)
+    module = GroupNormAct(4, 16).cuda()
+    for trace in (lambda: torch.jit.trace(lambda t: group_norm_act(t, 4), (x,), check_trace=False), lambda: torch.jit.trace(module, (x,)),
+                  lambda: make_fx(lambda t: group_norm_act(t, 4))(x), lambda: make_fx(lambda t: module(t))(x)):
+        with pytest.raises(NotImplementedError, match='traced'):
+            trace()
+        assert torch.equal(group_norm_act(x, 4), want)
+    leaf = x.detach().requires_grad_()
+    y = group_norm_act(leaf, 4, wt, b, residual=r)
+    with pytest.raises(NotImplementedError, match='traced'):
+        make_fx(lambda t: torch.autograd.grad(y, leaf, t, retain_graph=True)[0])(dy)
+    assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], _run(x, 4, wt, b, r, dy, 'relu')['dx'])

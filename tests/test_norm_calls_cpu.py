@@ -31,3 +31,25 @@ def test_functorch_transforms_are_refused():
                  lambda: torch.func.jvp(_entry, (x,), (x,)), lambda: torch.func.vmap(lambda t: _entry(x, t))(torch.ones(3, 4))):
         with pytest.raises(NotImplementedError, match='group_norm_act'):
             call()
+
+
+def test_tracing_is_refused():
+    """A trace would hold the result's allocation alone.  (The CPU statement is traced as ever.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x = torch.randn(2, 4, 3, 3)
+    for leaf in (x, x.clone().requires_grad_()):
+        with pytest.raises(NotImplementedError, match='traced'):
+            torch.jit.trace(_entry, (leaf,), check_trace=False)
+        for mode in ('real', 'fake', 'symbolic'):
+            with pytest.raises(NotImplementedError, match='traced'):
+                make_fx(lambda t: _entry(t), tracing_mode=mode)(leaf)
+    with FakeTensorMode():
+        fake = torch.empty(2, 4, 3, 3)
+        with pytest.raises(NotImplementedError, match='traced'):
+            _entry(fake)
+    with pytest.raises(NotImplementedError, match='memory of their own'):
+        _entry(fake)
+    traced = torch.jit.trace(lambda t: group_norm_act(t, 2), (x,), check_trace=False)
+    again = torch.randn(2, 4, 3, 3)
+    assert torch.equal(traced(again), group_norm_act(again, 2))
