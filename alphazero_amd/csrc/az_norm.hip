@@ -803,13 +803,13 @@ static void gn_plan_split(GnArgs& a, int VW, int dtype) {
     // to 32, 15.2 with up to 128)
     const long units = a.N * a.slices * a.pieces;
     long chunks = units ? (1024 + units - 1) / units : 1;
-    const long most = (a.HW + 4 * a.rstep - 1) / (4 * a.rstep);
+    const long most = ((long)a.HW + 4 * a.rstep - 1) / (4 * a.rstep);
     if (chunks > most) chunks = most;
     if (chunks > 32) chunks = 32;
     const long least = ((long)a.HW * a.C * gn_size(dtype) >> 31) + 1;         // (a chunk's offsets in 32 bits)
     if (chunks < least) chunks = least;
     a.rows = (int)((a.HW + chunks - 1) / chunks);
-    a.chunks = (a.HW + a.rows - 1) / a.rows;
+    a.chunks = (int)(((long)a.HW + a.rows - 1) / a.rows);                     // (HW + rows passes 2^31 in long samples)
 }
 
 // For the kernels that hold a sample's slice in registers: the team and K; false where no team can.

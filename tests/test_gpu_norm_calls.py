@@ -89,3 +89,37 @@ def test_tracing_is_refused_and_leaves_nothing_behind():
     with pytest.raises(NotImplementedError, match='traced'):
         make_fx(lambda t: torch.autograd.grad(y, leaf, t, retain_graph=True)[0])(dy)
     assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], _run(x, 4, wt, b, r, dy, 'relu')['dx'])
+
+
+@pytest.mark.parametrize('h,w', [(46340, 46340), (1, 2 ** 31 - 1)])
+def test_the_longest_samples(h, w):
+    """One channel of up to 2^31 - 1 values, all zero but for the last thousand, gradients there and in the first thousand.
+    Sums of the definition are those of the values that are not zero."""
+    from alphazero_amd.norm import group_norm_act
+    n, k = h * w, 1000
+    g = torch.Generator(device='cuda').manual_seed(35)
+    head, tail = (torch.randn(k, device='cuda', generator=g).bfloat16() for _ in range(2))
+    values = torch.randn(k, device='cuda', generator=g).bfloat16()
+    x, dy = (torch.zeros(1, 1, h, w, dtype=torch.bfloat16, device='cuda') for _ in range(2))
+    x.view(-1)[-k:] = values
+    dy.view(-1)[:k], dy.view(-1)[-k:] = head, tail
+    wt, b = torch.full((1,), 1.5, device='cuda', requires_grad=True), torch.full((1,), 0.25, device='cuda', requires_grad=True)
+    x.requires_grad_()
+    y = group_norm_act(x, 1, wt, b, act='none')
+    dx, dw, db = torch.autograd.grad(y, [x, wt, b], dy)
+    v, dh, dt = values.double(), head.double(), tail.double()
+    mean = v.sum() / n
+    rstd = 1 / torch.sqrt((v * v).sum() / n - mean * mean + 1e-5)
+    at_zero, at_v = -mean * rstd, (v - mean) * rstd
+    half = 2.0 ** -8
+    yv = y.detach().view(-1)
+    assert bool(((yv[-k:].double() - (1.5 * at_v + 0.25)).abs() <= half * (1.5 * at_v + 0.25).abs() + 1e-6 * (at_v.abs() + 1)).all())
+    assert bool((yv[:-k] == yv[0]).all()) and abs(yv[0].double() - (1.5 * at_zero + 0.25)) <= half
+    # (sums of 2000 terms, each rounded four times, in chains of no more than that)
+    terms, tol = torch.cat([dh * at_zero, dt * at_v]), 2010 * 2.0 ** -24
+    assert abs(dw[0].double() - terms.sum()) <= tol * terms.abs().sum()
+    assert abs(db[0].double() - (dh.sum() + dt.sum())) <= tol * (dh.abs().sum() + dt.abs().sum())
+    ma, mx = 1.5 * (dh.sum() + dt.sum()) / n, 1.5 * terms.sum() / n
+    for got, d, xhat in ((dx.view(-1)[:k], dh, at_zero), (dx.view(-1)[-k:], dt, at_v)):
+        want = rstd * (1.5 * d - ma - xhat * mx)
+        assert bool(((got.double() - want).abs() <= half * want.abs() + 1e-5 * rstd * (d.abs() + 1e-3)).all())

@@ -53,3 +53,24 @@ def test_tracing_is_refused():
     traced = torch.jit.trace(lambda t: group_norm_act(t, 2), (x,), check_trace=False)
     again = torch.randn(2, 4, 3, 3)
     assert torch.equal(traced(again), group_norm_act(again, 2))
+
+
+def _descriptor(**kw):
+    g = _lib.GroupNorm()
+    for k, v in dict(dict(batch=1, cells=9, channels=8, groups=4, act=1, eps=1e-5), **kw).items():
+        setattr(g, k, v)
+    return g
+
+
+def _workspace(backward, **kw):
+    import ctypes as C
+    return _lib.load().az_group_norm_workspace_bytes(C.byref(_descriptor(**kw)), backward)
+
+
+@pytest.mark.parametrize('cells', [46340 ** 2, 2 ** 31 - 1, 2 ** 31 - 31])
+@pytest.mark.parametrize('dtype', [0, 1])
+def test_workspace_of_the_longest_samples(cells, dtype):
+    """One channel, samples up to the limit of 2^31 - 1 values: 16 bytes of partial sums for each of at least two and at most
+    one chunk of 256 rows, and 8 for each in the backward pass."""
+    forward, backward = (_workspace(k, cells=cells, channels=1, groups=1, dtype=dtype) for k in (0, 1))
+    assert forward % 16 == 0 and 2 <= forward // 16 <= cells // 256 and backward == forward // 16 * 24
