@@ -501,9 +501,9 @@ k_gn_bwd_apply(GnArgs a) {
 // dw, db: the partial sums of `parts` workgroups, added in a fixed order in 64 bits.  One workgroup: 16 of the 2 C columns.
 // (2 to 4 us.  Not in the launch before it: a counter that finds the last workgroup would have to be kept, and cleared, between calls.)
 __global__ void __launch_bounds__(1024)
-k_gn_dparams(const float* __restrict__ dpart, long parts, int C, int wtype, void* dw, void* db) {
+k_gn_dparams(const float* __restrict__ dpart, long parts, int first, int C, int wtype, void* dw, void* db) {
     __shared__ double lds[64][17];
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
+    const int col = first + blockIdx.x * 16 + (threadIdx.x & 15), r0 = threadIdx.x >> 4;
     double s = 0.0;
     if (col < 2 * C)
 #pragma unroll 8
@@ -939,8 +939,13 @@ static void gn_held_t(const GnArgs& a, int VW, int dtype, bool backward, int K, 
     else gn_held_w<_Float16, SILU>(a, VW, backward, K, threads, st);
 }
 
+// HIP takes fewer than 2^32 work-items in a launch
+static bool gn_fits(long blocks, int threads) { return blocks > 0 && blocks * threads < (1l << 32); }
+static const char gn_too_many[] = "az_group_norm_act: the tensor takes 2^32 work-items or more, which is more than a launch";
+
 static int gn_held(const GnArgs& a, int VW, const az_group_norm* g, bool backward, int K, int threads, hipStream_t st) {
-    if (!backward && ((a.N + (1 << a.sb) - 1) >> a.sb) * a.slices > INT32_MAX) return az_fail("az_group_norm_act: more workgroups than a launch takes");
+    const long units = ((a.N + (1 << a.sb) - 1) >> a.sb) * a.slices, teams = a.tb == 6 ? threads / 64 : 1;
+    if (!gn_fits(backward ? (long)a.chunks * a.slices : (units + teams - 1) / teams, threads)) return az_fail(gn_too_many);
     if (g->act == AZ_ACT_SILU) gn_held_t<true>(a, VW, g->dtype, backward, K, threads, st);
     else gn_held_t<false>(a, VW, g->dtype, backward, K, threads, st);
     AZ_LAUNCH_CHECK("a group norm kernel");
@@ -976,7 +981,7 @@ static void gn_go_t(const GnArgs& a, int VW, int dtype, dim3 grid, hipStream_t s
 template <int STEP>
 static int gn_go(const GnArgs& a, int VW, const az_group_norm* g, hipStream_t st) {
     const long blocks = a.N * a.slices * a.pieces * a.chunks;
-    if (blocks > INT32_MAX) return az_fail("az_group_norm_act: more workgroups than a launch takes");
+    if (!gn_fits(blocks, GN_THREADS)) return az_fail(gn_too_many);                  // (both steps of a call have this grid)
     if (STEP > 0 && g->act == AZ_ACT_SILU) gn_go_t<STEP, true>(a, VW, g->dtype, dim3((unsigned)blocks), st);
     else gn_go_t<STEP, false>(a, VW, g->dtype, dim3((unsigned)blocks), st);
     AZ_LAUNCH_CHECK("a group norm kernel");
@@ -1057,8 +1062,11 @@ int az_group_norm_act_backward(const az_group_norm* g, const void* dy, const voi
         }
     }
     if (params) {
-        hipLaunchKernelGGL(k_gn_dparams, dim3((unsigned)((2 * a.C + 15) / 16)), dim3(1024), 0, st, a.dpart, parts, a.C, a.wtype, dweight, dbias);
-        AZ_LAUNCH_CHECK("k_gn_dparams");
+        for (int first = 0, most = 16 << 20; first < 2 * a.C; first += most) {       // (2^30 work-items at a time)
+            const int cols = 2 * a.C - first < most ? 2 * a.C - first : most;
+            hipLaunchKernelGGL(k_gn_dparams, dim3((unsigned)((cols + 15) / 16)), dim3(1024), 0, st, a.dpart, parts, first, a.C, a.wtype, dweight, dbias);
+            AZ_LAUNCH_CHECK("k_gn_dparams");
+        }
     }
     return 0;
 }

@@ -458,9 +458,10 @@ int  az_sgd_momentum_guarded(float* params, const float* grads, float* momentum_
  *   z = (x - mean) * rstd * weight[c] + bias[c] (+ residual),  y = act(z),
  * mean and rstd = 1 / sqrt(var + eps) over the cells and the channels / groups channels of a sample's group; sums and
  * statistics in 64 bits, the rest in 32, one rounding to the tensors' type.  relu and its gradient pass a NaN on.
- * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any size (a sample of at most
- * 2^31 - 1 values, 2^28 channels) and alignment (16-byte aligned tensors and groups of a multiple of 4 channels, 8 in 16
- * bits, run fastest).                                                                                              */
+ * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any alignment (16-byte aligned
+ * tensors and groups of a multiple of 4 channels, 8 in 16 bits, run fastest) and any size of up to 2^31 - 1 values a
+ * sample, 2^28 channels and 2^32 - 1 work-items in a launch (which tensors of some 10^9 values reach where groups have an
+ * odd number of channels, and of 10^10 otherwise).  A call that needs more is refused before anything is launched.   */
 #define AZ_F32  0
 #define AZ_BF16 1
 #define AZ_F16  2

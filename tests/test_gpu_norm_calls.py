@@ -123,3 +123,22 @@ def test_the_longest_samples(h, w):
     for got, d, xhat in ((dx.view(-1)[:k], dh, at_zero), (dx.view(-1)[-k:], dt, at_v)):
         want = rstd * (1.5 * d - ma - xhat * mx)
         assert bool(((got.double() - want).abs() <= half * want.abs() + 1e-5 * rstd * (d.abs() + 1e-3)).all())
+
+
+def test_more_channels_than_one_launch_of_parameter_gradients_takes():
+    """2^25 + 24 channels: two columns each for dweight and dbias.  Every group is the same eight values in another order of
+    channels' gradients, so the definition is that of one group."""
+    from alphazero_amd.norm import group_norm_act
+    c, groups = 2 ** 25 + 24, (2 ** 25 + 24) // 8
+    one = torch.tensor([-2.0, -1.0, -0.5, 0.0, 0.25, 0.5, 1.0, 3.0], device='cuda')
+    x = one.repeat(groups)[None].repeat(2, 1)
+    x[1] *= 2
+    x.requires_grad_()
+    wt, b = (torch.full((c,), v, device='cuda', requires_grad=True) for v in (1.0, 0.0))
+    scale = 1 + (torch.arange(c, device='cuda') % 1000).float() / 1000
+    dy = torch.stack([scale, -2 * scale])
+    dw, db = torch.autograd.grad(group_norm_act(x, groups, wt, b, act='none'), [wt, b], dy)
+    xhat = torch.stack([(k * one.double() - k * one.double().mean()) / torch.sqrt(k * k * one.double().var(correction=0) + 1e-5) for k in (1, 2)])
+    want = (xhat[0] - 2 * xhat[1]).repeat(groups) * scale.double()
+    assert bool(((dw.double() - want).abs() <= 20 * 2.0 ** -24 * 3 * xhat.abs().max() * scale).all())
+    assert torch.equal(db, -scale)

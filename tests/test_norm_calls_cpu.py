@@ -74,3 +74,22 @@ def test_workspace_of_the_longest_samples(cells, dtype):
     one chunk of 256 rows, and 8 for each in the backward pass."""
     forward, backward = (_workspace(k, cells=cells, channels=1, groups=1, dtype=dtype) for k in (0, 1))
     assert forward % 16 == 0 and 2 <= forward // 16 <= cells // 256 and backward == forward // 16 * 24
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason='asked where nothing could be launched')
+@pytest.mark.parametrize('big', [
+    dict(batch=2 ** 26, cells=1, channels=48, groups=16),                     # one channel a thread, held in registers
+    dict(batch=2 ** 26, cells=42, channels=128, groups=16),                   # the same, several
+    dict(batch=2 ** 24, cells=361, channels=512, groups=2),                   # teams of 1024
+    dict(batch=2 ** 22, cells=4096, channels=1024, groups=32),                # two passes
+    dict(batch=2 ** 31 - 1, cells=1, channels=64, groups=64)])
+def test_launches_of_too_many_work_items_are_refused(big):
+    """Before the first launch: no pointer here is one."""
+    import ctypes as C
+    lib, p = _lib.load(), C.c_void_p(256)
+    g = _descriptor(**big)
+    assert lib.az_group_norm_act(C.byref(g), p, None, None, None, p, None, p, 1 << 60, None) != 0
+    assert b'work-items' in lib.az_last_error()
+    if big['cells'] == 4096:
+        assert lib.az_group_norm_act_backward(C.byref(g), p, p, None, None, None, p, p, p, p, None, p, 1 << 60, None) != 0
+        assert b'work-items' in lib.az_last_error()
