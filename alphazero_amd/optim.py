@@ -3,8 +3,8 @@
 FlatSGD: torch.optim.SGD as the reference configures it (alphazero/training.py:27-29: momentum, weight
 decay) with the whole update in ONE launch of az_sgd_momentum (csrc/az_train.hip).
 
-All parameters are moved into one flat fp32 buffer (each parameter becomes a view of it, so the module, its
-state_dict and everything that reads the weights keep working), gradients accumulate into a second flat buffer
+All parameters are moved into one flat fp32 buffer (each parameter becomes a view of it, channels last where it was,
+so the module, its state_dict and everything that reads the weights keep working), gradients accumulate into a second flat buffer
 through persistent `.grad` views, and the momentum is a third.  A step is then a single kernel over n elements
 instead of three small launches per tensor.  It is a torch Optimizer, so MultiStepLR drives its learning rate
 exactly as it drives SGD's (training.py:30-31)."""
@@ -13,6 +13,13 @@ import ctypes as C
 import torch
 
 from . import _lib
+
+
+def _strided_like(flat, p):
+    """`flat` (p.numel() elements) in the shape of p, in p's order of memory where that is dense."""
+    if p.dim() == 4 and not p.is_contiguous() and p.is_contiguous(memory_format=torch.channels_last):
+        return flat.as_strided(p.shape, p.stride(), flat.storage_offset())
+    return flat.view(p.shape)
 
 
 class FlatSGD(torch.optim.Optimizer):
@@ -38,9 +45,10 @@ class FlatSGD(torch.optim.Optimizer):
         with torch.no_grad():
             for p in uniq:
                 k = p.numel()
-                self.flat_p[off:off + k].copy_(p.reshape(-1))
-                p.data = self.flat_p[off:off + k].view_as(p)
-                p.grad = self.flat_g[off:off + k].view_as(p)
+                at_p = _strided_like(self.flat_p[off:off + k], p)
+                at_p.copy_(p)
+                p.grad = _strided_like(self.flat_g[off:off + k], p)
+                p.data = at_p
                 off += k
         self._steps = 0
         self.withheld = torch.zeros(1, dtype=torch.int32, device=dev)   # recorded steps whose update the guard refused
@@ -92,13 +100,6 @@ class FlatSGD(torch.optim.Optimizer):
                                                             float(g['weight_decay']), _lib.ptr(guard), float(guard_limit),
                                                             _lib.ptr(self.withheld), st))
         self._steps += 1
-
-
-def _strided_like(flat, p):
-    """`flat` (p.numel() elements) in the shape of p, in p's order of memory where that is dense."""
-    if p.dim() == 4 and not p.is_contiguous() and p.is_contiguous(memory_format=torch.channels_last):
-        return flat.as_strided(p.shape, p.stride(), flat.storage_offset())
-    return flat.view(p.shape)
 
 
 class FlatAdamW(torch.optim.Optimizer):

@@ -12,6 +12,8 @@ from device memory (AZ_TRAIN_GRAPH=0 or record_step=False keeps every step eager
 writer and model server are duck-typed (`add_scalar`, `update(model, version)`).  `dataset` is a
 ReplayBufferDataset (the reference's per-state sample dicts) or a DeviceReplayWindow (batches taken
 straight from tensors on the GPU)."""
+import os
+
 import numpy as np
 import torch
 import torch.nn.functional as F
@@ -36,6 +38,13 @@ class TrainingWorker:
         self._writer, self._device, self._num_workers = summary_writer, device, num_workers
         self._model = config.Model().to(device)
         self._loss = config.Loss()
+        hand = False
+        if torch.device(device).type == 'cuda' and os.environ.get('AZ_TRAIN_HANDWRITTEN', '1') != '0' and self._batch_size >= 2:
+            from . import train_c4
+            from .loss import AlphaZeroLoss
+            hand = train_c4.supports(self._model) and type(self._loss) is AlphaZeroLoss
+            if hand:
+                self._model.to(memory_format=torch.contiguous_format)      # (how its kernels read the weights)
         t = config.training
         # training.optimizer: 'sgd' as the reference (the default), or 'adamw' with betas, eps, state_bits (32, or 8 on
         # the GPU) and seed
@@ -64,7 +73,6 @@ class TrainingWorker:
         self._lr_schedule = MultiStepLR(self._optimizer, t['lr_schedule'], gamma=t['lr_schedule_gamma'])
         self._sampler = ReplayBufferSampler(dataset, batch_size=self._batch_size, bufferlen=64 * 1024)
         self._iter = 0
-        import os
         if record_step is None:
             record_step = os.environ.get('AZ_TRAIN_GRAPH', '1') != '0'
         self._record = bool(record_step and torch.device(device).type == 'cuda' and hasattr(dataset, 'sample_into')
@@ -78,13 +86,8 @@ class TrainingWorker:
                 and dataset.kernel_sampling(self._batch_size)):
             self._sample_seed = None           # drawn from torch's generator at the first batch (see _seed())
             self._draw = torch.zeros(1, dtype=torch.int64, device=device)
-        # the hand-written pass binds the parameters and their .grad tensors where FlatSGD has put them
-        self._hand = None
-        if torch.device(device).type == 'cuda' and os.environ.get('AZ_TRAIN_HANDWRITTEN', '1') != '0' and self._batch_size >= 2:
-            from . import train_c4
-            from .loss import AlphaZeroLoss
-            if train_c4.supports(self._model) and type(self._loss) is AlphaZeroLoss:
-                self._hand = train_c4.C4TrainStep(self._model)
+        # the hand-written pass binds the parameters and their .grad tensors where the optimizer has put them
+        self._hand = train_c4.C4TrainStep(self._model) if hand else None
 
     @property
     def model(self):
