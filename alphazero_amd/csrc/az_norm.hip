@@ -29,6 +29,7 @@
 #include "az_host.h"
 
 #define GN_THREADS 256
+#define GN_CHAIN 2048         // rows that a thread adds up in 32 bits for dweight and dbias, at most; all sums of such sums in 64
 
 struct GnArgs {
     const void* x; const void* dy; const void* res; const void* w; const void* b;
@@ -453,9 +454,9 @@ k_gn_bwd_sums(GnArgs a) {
     __syncthreads();
     for (int o = threadIdx.x; o < 2 * VW * p.width; o += GN_THREADS) {
         const int t = o % p.width, v = o / p.width, col = t % a.cw + p.piece * a.cw, g = p.g - p.gl + t / a.cw;
-        float total = 0.0f;
+        double total = 0.0;
         for (int r = 0; r < a.rstep; ++r) total += sums[v][r * p.width + t];
-        if (col < a.cpg && g < a.G) a.dpart[((p.n * a.chunks + p.chunk) * 2 + (v & 1)) * a.C + g * a.Cg + col * VW + (v >> 1)] = total;
+        if (col < a.cpg && g < a.G) a.dpart[((p.n * a.chunks + p.chunk) * 2 + (v & 1)) * a.C + g * a.Cg + col * VW + (v >> 1)] = (float)total;
     }
 }
 
@@ -608,9 +609,9 @@ k_gn_held(GnArgs a) {
 
 // a workgroup's sum for one channel: v = 2 * (channel of the vector) + (0: db, 1: dw)
 template <int VW>
-__device__ __forceinline__ void gn_put_param(const GnArgs& a, int slice, int walker, int t, int v, float total) {
+__device__ __forceinline__ void gn_put_param(const GnArgs& a, int slice, int walker, int t, int v, double total) {
     const int col = t & ((1 << a.cb) - 1), g = (slice << a.gb) + (t >> a.cb);
-    if (col < a.cpg && g < a.G) a.dpart[((long)walker * 2 + (v & 1)) * a.C + g * a.Cg + col * VW + (v >> 1)] = total;
+    if (col < a.cpg && g < a.G) a.dpart[((long)walker * 2 + (v & 1)) * a.C + g * a.Cg + col * VW + (v >> 1)] = (float)total;
 }
 
 // A team walks over the samples of its slice, so that dw and db stay in its registers; the teams of a workgroup have the
@@ -621,7 +622,8 @@ template <typename T, int VW, int K, int THREADS, bool SILU>
 __global__ void __launch_bounds__(THREADS)
 k_gn_bwd_held(GnArgs a) {
     typedef typename GnVec<T, VW>::type V;
-    __shared__ float lds[THREADS][2], sums[2 * VW][THREADS];
+    __shared__ float lds[THREADS][2];
+    __shared__ alignas(8) float sums[2 * VW][THREADS];
     const bool alone = a.tb == 6;
     const unsigned block = gn_block(a);
     const int slice = block % a.slices, walker0 = block / a.slices;
@@ -714,20 +716,20 @@ k_gn_bwd_held(GnArgs a) {
     for (int i = 0; i < VW; ++i) { sums[2 * i][threadIdx.x] = db[i]; sums[2 * i + 1][threadIdx.x] = dw[i]; }
     __syncthreads();
     const int share = outs >= THREADS ? 1 : min(16, THREADS / outs);
-    float total = 0.0f;
+    double total = 0.0;
     for (int o = threadIdx.x; o < outs * share; o += THREADS) {
         const int t = o & keep, v = (o >> bits) % (2 * VW), part = o / outs;
-        total = 0.0f;
+        total = 0.0;
         for (int r = t + (part << bits); r < THREADS; r += share << bits) total += sums[v][r];
         if (share == 1) gn_put_param<VW>(a, slice, walker0, t, v, total);
     }
     if (share == 1) return;
     __syncthreads();
-    float* flat = &sums[0][0];
+    double* flat = reinterpret_cast<double*>(&sums[0][0]);            // (outs * share <= THREADS of them)
     if (threadIdx.x < outs * share) flat[threadIdx.x] = total;
     __syncthreads();
     if (threadIdx.x < outs) {
-        total = 0.0f;
+        total = 0.0;
         for (int part = 0; part < share; ++part) total += flat[part * outs + threadIdx.x];
         gn_put_param<VW>(a, slice, walker0, threadIdx.x & keep, (int)threadIdx.x >> bits, total);
     }
@@ -806,7 +808,8 @@ static void gn_plan_split(GnArgs& a, int VW, int dtype) {
     const long most = ((long)a.HW + 4 * a.rstep - 1) / (4 * a.rstep);
     if (chunks > most) chunks = most;
     if (chunks > 32) chunks = 32;
-    const long least = ((long)a.HW * a.C * gn_size(dtype) >> 31) + 1;         // (a chunk's offsets in 32 bits)
+    long least = ((long)a.HW * a.C * gn_size(dtype) >> 31) + 1;               // (a chunk's offsets in 32 bits)
+    if (least * a.rstep * GN_CHAIN < a.HW) least = ((long)a.HW + a.rstep * GN_CHAIN - 1) / (a.rstep * GN_CHAIN);
     if (chunks < least) chunks = least;
     a.rows = (int)((a.HW + chunks - 1) / chunks);
     a.chunks = (int)(((long)a.HW + a.rows - 1) / a.rows);                     // (HW + rows passes 2^31 in long samples)
@@ -872,6 +875,8 @@ static bool gn_plan_held(GnArgs& a, int VW, int dtype, bool silu, bool backward,
                 const long most_rows = a.N * a.HW * gn_size(dtype) * 3 / 128;
                 if (blocks > 1536 / slices) blocks = 1536 / slices;
                 if (blocks > most_rows) blocks = most_rows;
+                const long least = (batches * K + teams * GN_CHAIN - 1) / (teams * GN_CHAIN);
+                if (blocks < least) blocks = least;
                 if (blocks > (batches + teams - 1) / teams) blocks = (batches + teams - 1) / teams;
                 if (blocks < 1) blocks = 1;
                 a.walkers = (int)(blocks * teams);

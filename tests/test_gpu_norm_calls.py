@@ -142,3 +142,17 @@ def test_more_channels_than_one_launch_of_parameter_gradients_takes():
     want = (xhat[0] - 2 * xhat[1]).repeat(groups) * scale.double()
     assert bool(((dw.double() - want).abs() <= 20 * 2.0 ** -24 * 3 * xhat.abs().max() * scale).all())
     assert torch.equal(db, -scale)
+
+
+@pytest.mark.parametrize('shape', [(1, 255, 1024, 1024), (40000, 3, 19, 19)])
+def test_long_sums_of_equal_terms(shape):
+    """Equal gradients, whose float32 sum is rounded the same way at every step: n of them added in one chain are off by n / 6
+    half steps.  2048 rows at most are added so, the rest in 64 bits."""
+    from alphazero_amd.norm import group_norm_act
+    n, c, h, w = shape
+    x = torch.zeros(shape, device='cuda').contiguous(memory_format=torch.channels_last)
+    b = torch.zeros(c, device='cuda', requires_grad=True)
+    dy = torch.full_like(x, 0.3)
+    (db,) = torch.autograd.grad(group_norm_act(x, 1, None, b, act='none'), [b], dy)
+    want = n * h * w * dy[0, 0, 0, 0].double()
+    assert bool(((db.double() - want).abs() <= (2048 + 1) * 2.0 ** -24 * want).all())

@@ -93,3 +93,16 @@ def test_launches_of_too_many_work_items_are_refused(big):
     if big['cells'] == 4096:
         assert lib.az_group_norm_act_backward(C.byref(g), p, p, None, None, None, p, p, p, p, None, p, 1 << 60, None) != 0
         assert b'work-items' in lib.az_last_error()
+
+
+@pytest.mark.parametrize('case', [dict(batch=2 ** 24, cells=42, channels=256, groups=32), dict(batch=2 ** 23, cells=361, channels=192, groups=16, dtype=1),
+                                  dict(batch=1, cells=2 ** 20, channels=255, groups=1), dict(batch=1, cells=2 ** 23, channels=255, groups=1, dtype=2)])
+def test_parameter_gradients_are_added_in_chains_of_2048_rows(case):
+    """What that takes at the least: a workgroup of at most 1024 threads that hold 16 bytes of a row each, and add 2048 of them
+    up, ends in one row of partial sums for its channels."""
+    size = 4 if case.get('dtype', 0) == 0 else 2
+    rows = _workspace(1, **case) // (8 * case['channels'])
+    one = 1024 * 2048 * (16 // size) // case['channels']
+    if case['batch'] == 1:
+        one = 2048 * 256 // 255                    # (an odd number of channels: one to a thread, 256 threads)
+    assert rows >= case['batch'] * case['cells'] // one
