@@ -156,3 +156,46 @@ def test_long_sums_of_equal_terms(shape):
     (db,) = torch.autograd.grad(group_norm_act(x, 1, None, b, act='none'), [b], dy)
     want = n * h * w * dy[0, 0, 0, 0].double()
     assert bool(((db.double() - want).abs() <= (2048 + 1) * 2.0 ** -24 * want).all())
+
+
+@pytest.mark.parametrize('shape', [(3, 32, 4, 6, 7), (2, 30, 5, 5, 3), (3, 48, 4, 19, 19), (2, 64, 8, 32, 32), (1, 320, 32, 64, 64), (4, 24, 4, 1, 1)])
+@pytest.mark.parametrize('offset', [1e5, -1e6])
+@pytest.mark.parametrize('act', ['none', 'relu'])
+def test_means_that_are_large_against_the_spread(shape, offset, act):
+    """float32 values 10^5 and 10^6 spreads from zero, within the tolerances of any others."""
+    n, c, groups, h, w = shape
+    x, wt, b, r, dy = _inputs(n, c, h, w, torch.float32, torch.float32, True, 36, offset)
+    want, tol = _reference(x, groups, wt, b, r, dy, act)
+    _check(_run(x, groups, wt, b, r, dy, act), want, tol, torch.float32, torch.float32)
+
+
+@pytest.mark.parametrize('shape', [(4, 16, 2, 6, 7), (2, 64, 8, 32, 32), (1, 6, 2, 100, 101), (5, 8, 1, 1, 1)])
+@pytest.mark.parametrize('value', [1.0, -12345.678, 1e-3])
+def test_groups_equal_but_for_one_last_bit_without_an_eps(shape, value):
+    """eps = 0 and one value a half step away: the variance is (n - 1) / n^2 of that step's square and not zero."""
+    n, c, groups, h, w = shape
+    x = torch.full((n, c, h, w), value, device='cuda').contiguous(memory_format=torch.channels_last)
+    per = c // groups
+    for g in range(groups):
+        for s in range(n):                                             # the first value of the group, the last, one within
+            at = (g * per + (0, per - 1, per // 2)[s % 3], (0, h - 1, h // 2)[s % 3], (0, w - 1, w // 2)[s % 3])
+            x[s][at] = torch.nextafter(x[s][at], torch.tensor(float('inf' if s % 2 else '-inf'), device='cuda'))
+    wt, b, dy = torch.ones(c, device='cuda'), torch.zeros(c, device='cuda'), torch.randn(n, c, h, w, device='cuda').contiguous(memory_format=torch.channels_last)
+    # The reference goes by x less `value`, which is exact and changes nothing: the mean of x itself lies a thousandth of a half
+    # step from `value`, and no 64-bit number is nearer to it than 2^-53 of it.  That is what the kernel's mean is off by (half
+    # a unit in the last place, where the first value and the mean's distance from it are added), and y by as much times
+    # rstd: n / sqrt(n - 1) over the step of at least 2^-24 |value| makes it 2^-29 sqrt(n), some 2^-24 of values of 1 / sqrt(n).
+    want, tol = _reference(x - x.new_tensor(value), groups, wt, b, None, dy, 'none', eps=0.0)
+    got = _run(x, groups, wt, b, None, dy, 'none', eps=0.0)
+    count = per * h * w
+    tol['y'] = tol['y'] + 2.0 ** -29 * count / (count - 1) ** 0.5
+    assert all(bool(v.isfinite().all()) for v in got.values())
+    _check(got, want, tol, torch.float32, torch.float32)
+
+
+def test_a_first_value_far_from_its_group():
+    """Sums are taken from the group's first value: here it lies a million spreads of the others away."""
+    x, wt, b, r, dy = _inputs(4, 32, 6, 7, torch.float32, torch.float32, True, 37)
+    x[:, ::8, 0, 0] = torch.tensor([1e6, -1e6, 1e3, -3e4], device='cuda')[:, None]
+    want, tol = _reference(x, 4, wt, b, r, dy, 'relu')
+    _check(_run(x, 4, wt, b, r, dy, 'relu'), want, tol, torch.float32, torch.float32)
