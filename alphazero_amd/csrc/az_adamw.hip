@@ -3,7 +3,7 @@
 //
 //   t = t + 1
 //   m = (b1 * m) + ((1 - b1) * g)          v = (b2 * v) + ((1 - b2) * (g * g))
-//   p = p * (1 - lr * wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//   p = p * (1 - lr * wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)        (0 / 0, where eps is 0, taken as 0)
 //
 // The tensors lie behind each other in flat buffers, each from a multiple of 256 elements on (the gaps are zero and stay
 // zero); tensors with the same settings form a run.  The step count lives in device memory, so that a launch recorded
@@ -229,7 +229,11 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
                 p[i] = p[i] * s.keep - s.step * m[i] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[i]) * s.root + s.eps);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = p[i] * s.keep - s.step * m[i] / (sqrtf(v[i]) * s.root + s.eps);
+            for (int i = 0; i < 4; ++i) {
+                // (0 / 0 without an eps: no update, in the gaps and where every gradient was zero)
+                const float den = sqrtf(v[i]) * s.root + s.eps;
+                p[i] = p[i] * s.keep - (den == 0.0f && m[i] == 0.0f ? 0.0f : s.step * m[i] / den);
+            }
         }
         *reinterpret_cast<f32x4*>(q.p + at) = p;
         if (s.half) *reinterpret_cast<bf16x4*>(q.p16 + at) = __builtin_convertvector(p, bf16x4);

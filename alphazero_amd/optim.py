@@ -104,7 +104,8 @@ class FlatSGD(torch.optim.Optimizer):
 
 class FlatAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW (decoupled weight decay, bias correction; no amsgrad) with the whole update of all parameter
-    groups in ONE launch of az_adamw_step (csrc/az_adamw.hip), beside FlatSGD.
+    groups in ONE launch of az_adamw_step (csrc/az_adamw.hip), beside FlatSGD.  With eps=0 an element that has had no
+    gradient but zero has no update (torch's is 0 / 0).
 
     All parameters that require gradients at construction move into one flat buffer (each becomes a view of it, padded to 256
     elements), gradients accumulate into a second through persistent `.grad` views (use this class's zero_grad; a

@@ -495,6 +495,7 @@ int  az_group_norm_act_backward(const az_group_norm* g, const void* dy, const vo
  * form a run of blocks.  Per element, t = step + 1:
  *   m = (beta1 * m) + ((1 - beta1) * g);  v = (beta2 * v) + ((1 - beta2) * (g * g));
  *   p = p * (1 - lr * weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * (with eps 0 an element whose m and v are 0 has no update: the gaps stay zero).
  * p is float32 everywhere; in a run with half != 0 the parameters and gradients are bfloat16 (p16, g16) and p is their
  * master copy, p16 its rounding (a p16 that is not was written by somebody else, and the master becomes it).  state_bits 32: m, v float32.  state_bits 8: m8, v8 one byte per element and
  * top uint16[blocks][2], 11 leading float bits of each block's largest |m| and v (format and rounding: csrc/az_adamw.hip);
