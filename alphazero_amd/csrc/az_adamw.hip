@@ -43,7 +43,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 struct AdamwRun { long first_block; double lr, beta1, beta2, log1, log2, eps, weight_decay; int half, lr_index; };
 struct AdamwRuns { AdamwRun r[AZ_ADAMW_MAX_RUNS]; int n; };
-struct AdamwScalars { float keep, step, root, b1, c1, b2, c2, eps; int half; };
+struct AdamwScalars { float keep, step, root, b1, c1, b2, c2, eps; int half, fast; };
 
 __device__ __forceinline__ uint64_t adamw_mix(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
@@ -195,6 +195,10 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
         s.b1 = (float)r.beta1; s.c1 = (float)(1.0 - r.beta1);
         s.b2 = (float)r.beta2; s.c2 = (float)(1.0 - r.beta2);
         s.eps = (float)r.eps; s.half = r.half;
+        // The hardware's square root and reciprocal are good to 2^-23, but the root takes a subnormal number for zero: up to
+        // 2^-63, which is root times that in the denominator, half a step of eps or less where eps is 2^-39 root and more (with
+        // the customary betas and an eps of 1e-8 at every step; an eps of 1e-12 never, whose steps take IEEE's functions).
+        s.fast = s.eps >= s.root * 0x1p-39f;
         sc[tid] = s;
     }
     __syncthreads();
@@ -221,9 +225,7 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
             m[i] = m[i] * s.b1 + g[i] * s.c1;
             v[i] = v[i] * s.b2 + (g[i] * g[i]) * s.c2;
         }
-        // The hardware's square root and reciprocal are good to 2^-23 but take a subnormal number for zero: next to an
-        // eps of 2^-40 and more neither can be told apart from the exact ones.
-        if (s.eps >= 0x1p-40f) {
+        if (s.fast) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 p[i] = p[i] * s.keep - s.step * m[i] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[i]) * s.root + s.eps);

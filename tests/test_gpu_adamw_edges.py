@@ -1,6 +1,7 @@
 """FlatAdamW at the edges of its formula: no eps, denominators next to nothing, 8-bit moments of bfloat16 parameters.
 
 Tolerances: test_gpu_adamw.py, whose statement of the 8-bit format is used here."""
+import numpy as np
 import pytest
 import torch
 
@@ -42,3 +43,21 @@ def test_without_an_eps_what_never_had_a_gradient_stays(bits, dtype):
             for _ in range(3):
                 want = want * (1 - 1e-2 * 0.1) - size
             assert bool(((value - want)[~idle].abs() <= 3 * 20 * U * (p0.double().abs() + 0.03)[~idle]).all())
+
+
+@pytest.mark.parametrize('eps', [2.0 ** -40, 2.0 ** -36, 1e-10, 1e-8])
+@pytest.mark.parametrize('betas', [(0.9, 0.999), (0.9, 0.9999999), (0.9, 0.5)])
+def test_second_moments_below_the_smallest_normal_number(eps, betas):
+    """v is subnormal after a first gradient of 10^-18, and its root, over the correction, is as large as the gradient:
+    4e-6 of an eps of 2^-40.  p starts at 0, so that the update is the result: 16 roundings of it, and those of v (four; its
+    last bit is 2^-149, and the smallest v that is looked at 2^-130)."""
+    from alphazero_amd.optim import FlatAdamW
+    p = [torch.nn.Parameter(torch.zeros(1024, device='cuda'))]
+    opt = FlatAdamW(p, lr=1.0, betas=betas, eps=eps, weight_decay=0.0)
+    c2 = 1 - betas[1]
+    g = torch.logspace(np.log10(2.0 ** -65 / c2 ** 0.5), np.log10(2.0 ** -60 / c2 ** 0.5), 1024).cuda()
+    p[0].grad.copy_(g)
+    opt.step()
+    want = -g.double() / (g.double() + eps)
+    # (g's own square, rounded, against the last bit of a subnormal number: 2^-20 of v at 2^-130, half of that in its root)
+    assert bool(((p[0].detach().double() - want).abs() <= (20 * U + 2.0 ** -21 * g.double() / (g.double() + eps)) * want.abs()).all())
