@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_adamw import SIZES, U, _grads, _params
+from test_gpu_adamw import SIZES, U, _decode, _encode, _grads, _params, _random16
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +61,34 @@ def test_second_moments_below_the_smallest_normal_number(eps, betas):
     want = -g.double() / (g.double() + eps)
     # (g's own square, rounded, against the last bit of a subnormal number: 2^-20 of v at 2^-130, half of that in its root)
     assert bool(((p[0].detach().double() - want).abs() <= (20 * U + 2.0 ** -21 * g.double() / (g.double() + eps)) * want.abs()).all())
+
+
+@pytest.mark.parametrize('sizes', [SIZES, [(700, 300)]])
+def test_8_bit_moments_of_bfloat16_parameters_bit_for_bit(sizes):
+    """Codes and tops after each of five steps against the definition, from bfloat16 gradients; the masters against 64 bits, the
+    parameters their roundings."""
+    from alphazero_amd.optim import FlatAdamW
+    params = _params(sizes, 4, torch.bfloat16)
+    opt = FlatAdamW(params, lr=1e-2, state_bits=8, seed=2 ** 62 + 99)
+    f = np.float32
+    rows = lambda t: t.float().cpu().numpy().reshape(-1, 256)
+    for k in range(5):
+        for p, g in zip(params, _grads(params, 60 + k)):
+            p.grad.copy_(g)
+        g, p0 = rows(opt.flat_g16), rows(opt.flat_p)
+        m0, v0 = (rows(t) for t in opt.state_values())
+        opt.step()
+        m = m0 * f(0.9) + g * f(1 - 0.9)
+        v = v0 * f(0.999) + (g * g) * f(1 - 0.999)
+        rm, rv = _random16(opt.seed, k + 1, m.shape[0])
+        cm, tm = _encode(m, rm, 127)
+        cv, tv = _encode(v, rv, 255)
+        assert np.array_equal(opt.codes_m.cpu().numpy().reshape(-1, 256), cm), k
+        assert np.array_equal(opt.codes_v.cpu().numpy().reshape(-1, 256), cv), k
+        assert np.array_equal(opt.tops.cpu().numpy().reshape(-1, 2), np.concatenate([tm, tv], 1)), k
+        gm, gv = (rows(t) for t in opt.state_values())
+        assert np.array_equal(gm, _decode(cm, tm, 127)) and np.array_equal(gv, _decode(cv, tv, 255))
+        up = 1e-2 / (1 - 0.9 ** (k + 1)) * m.astype(np.float64) / (np.sqrt(v.astype(np.float64)) / np.sqrt(1 - 0.999 ** (k + 1)) + 1e-8)
+        want = p0.astype(np.float64) * (1 - 1e-2 * 1e-2) - up
+        assert np.all(np.abs(rows(opt.flat_p) - want) <= 3 * U * np.abs(p0) + 16 * U * np.abs(up))
+        assert torch.equal(opt.flat_p.to(torch.bfloat16), opt.flat_p16)

@@ -199,3 +199,17 @@ def test_a_first_value_far_from_its_group():
     x[:, ::8, 0, 0] = torch.tensor([1e6, -1e6, 1e3, -3e4], device='cuda')[:, None]
     want, tol = _reference(x, 4, wt, b, r, dy, 'relu')
     _check(_run(x, 4, wt, b, r, dy, 'relu'), want, tol, torch.float32, torch.float32)
+
+
+@pytest.mark.parametrize('dtype,param', [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16)])
+@pytest.mark.parametrize('shape', [(6, 32, 4, 6, 7), (2, 64, 8, 32, 32), (3, 48, 4, 19, 19), (3, 320, 32, 64, 64)])
+@pytest.mark.parametrize('act', ['relu', 'silu'])
+def test_weight_and_bias_off_any_border(dtype, param, shape, act):
+    """Both, or one of them, one value off a 16-byte border, as in a buffer without gaps: the bits of aligned ones."""
+    n, c, groups, h, w = shape
+    x, wt, b, r, dy = _inputs(n, c, h, w, dtype, param, True, 38)
+    want = _run(x, groups, wt, b, r, dy, act)
+    odd = lambda t, k: torch.empty(c + 8, dtype=param, device='cuda')[k:k + c].copy_(t)
+    for kw, kb in ((1, 1), (3, 0), (0, 1)):
+        got = _run(x, groups, odd(wt, kw), odd(b, kb), r, dy, act)
+        assert all(torch.equal(got[k], want[k]) for k in want), (kw, kb)
