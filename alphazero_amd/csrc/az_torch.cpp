@@ -52,7 +52,8 @@ void plain(const Tensor& t) {
 void untraced() {
     using c10::impl::TorchDispatchModeTLS;
     TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
-                                    !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::FAKE),
+                                    !TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::FAKE) &&
+                                    !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),
                                 "group_norm_act cannot be traced on the GPU (torch.jit.trace, make_fx, torch.export, fake tensors)");
 }
 
@@ -123,8 +124,8 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
             const int64_t channels = dy_.size(1);
             same(x_, dy_, dy_.sizes(), dy_.scalar_type());
             if (r_.defined()) same(r_, dy_, dy_.sizes(), dy_.scalar_type());
-            for (const Tensor& t : {w_, b_})
-                if (t.defined()) same(t, dy_, {channels}, t.scalar_type() == at::kFloat ? at::kFloat : dy_.scalar_type());
+            for (const Tensor* t : {&w_, &b_})
+                if (t->defined()) same(*t, dy_, {channels}, t->scalar_type() == at::kFloat ? at::kFloat : dy_.scalar_type());
             TORCH_CHECK(!w_.defined() || !b_.defined() || w_.scalar_type() == b_.scalar_type(), "group_norm_act: weight and bias of two types were saved");
             same(stats_, dy_, {dy_.size(0), groups, 2}, at::kDouble);
             const Tensor x = last(x_), residual = r_.defined() ? last(r_) : r_, weight = w_.defined() ? w_.contiguous() : w_,
@@ -153,7 +154,7 @@ Tensor group_norm_act(const Tensor& x, const std::optional<Tensor>& weight, cons
                       const std::optional<Tensor>& residual, int64_t groups, double eps, int64_t act) {
     const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
     untraced();
-    for (const Tensor& t : {x, w, b, r}) plain(t);
+    for (const Tensor* t : {&x, &w, &b, &r}) plain(*t);
     const bool grad = at::GradMode::is_enabled() &&
                       (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()) || (r.defined() && r.requires_grad()));
     if (grad) return GroupNormAct::apply(x, weight, bias, residual, groups, eps, act);

@@ -44,6 +44,8 @@ def test_tracing_is_refused():
         for mode in ('real', 'fake', 'symbolic'):
             with pytest.raises(NotImplementedError, match='traced'):
                 make_fx(lambda t: _entry(t), tracing_mode=mode)(leaf)
+            with pytest.raises(NotImplementedError, match='traced'):
+                make_fx(lambda t: _entry(t), tracing_mode=mode, pre_dispatch=True)(leaf)
     with FakeTensorMode():
         fake = torch.empty(2, 4, 3, 3)
         with pytest.raises(NotImplementedError, match='traced'):
