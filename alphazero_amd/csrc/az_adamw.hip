@@ -7,7 +7,7 @@
 //
 // The tensors lie behind each other in flat buffers, each from a multiple of 256 elements on (the gaps are zero and stay
 // zero); tensors with the same settings form a run.  The step count lives in device memory, so that a launch recorded
-// in a HIP graph counts on: every workgroup reads it first, the last one to finish writes it.
+// in a HIP graph counts on: one counter for each workgroup, which reads it first and writes it back one higher.
 //
 // Moments in 8 bits, for each block of 256 elements: `top` = the 11 leading bits of a float (exponent, 3 bits of
 // mantissa) of the block's largest magnitude, rounded up, and per element how many such steps below the top it is:
@@ -29,11 +29,11 @@
 #define ADAMW_BLOCK AZ_ADAMW_BLOCK   // elements: four of each lane of a wave
 static_assert(ADAMW_BLOCK == 4 * 64, "a wave takes a block");
 // A wave takes a block, four neighbouring elements to a lane, so that every load and store of a wave is one piece of memory.
-// Bound by memory in 32 bits (28 bytes an element): 46 M parameters 222 us = 5.8 TB/s, where a copy of as much has 4.7 to
-// 5.2.  In 8 bits (16 bytes) by memory and instructions alike: 129 us = 5.7 TB/s, and 77 vector instructions an element
-// keep the SIMDs busy for 69 % of it, the random numbers about a sixth of them.  Workgroups of 512 threads that take one
-// block a wave and end: their traffic moves along memory as one front.  2048 workgroups that walk over the blocks: 238 to
-// 250 and 137 to 146 us.
+// Bound by memory in 32 bits (28 bytes an element): 46 M parameters 223 us = 5.8 TB/s, where a copy of as much has 4.7 to
+// 5.2.  In 8 bits (16 bytes) by memory and instructions alike: 138 us = 5.4 TB/s, and 77 vector instructions an element
+// keep the SIMDs busy for 69 % of it, the random numbers about a sixth of them.  Workgroups of 512 threads whose waves take
+// one block and end, or, beyond 33.5 M elements (AZ_ADAMW_STEPS workgroups), walk in steps of the whole grid: their traffic
+// moves along memory as one front.  2048 workgroups that walk took 238 to 250 us beside 222, and 137 to 146 beside 129.
 #define ADAMW_THREADS 512
 #define ADAMW_GOLDEN 0x9E3779B97F4A7C15ull
 
@@ -197,7 +197,8 @@ k_adamw(az_adamw_buffers q, long blocks, AdamwRuns runs, const double* __restric
         s.eps = (float)r.eps; s.half = r.half;
         // The hardware's square root and reciprocal are good to 2^-23, but the root takes a subnormal number for zero: up to
         // 2^-63, which is root times that in the denominator, half a step of eps or less where eps is 2^-39 root and more (with
-        // the customary betas and an eps of 1e-8 at every step; an eps of 1e-12 never, whose steps take IEEE's functions).
+        // the customary betas and an eps of 1e-8 at every step; an eps of 1e-12 never, whose steps take IEEE's functions:
+        // 46 M parameters in 8 bits 143 us for 131, in 32 bits the same).
         s.fast = s.eps >= s.root * 0x1p-39f;
         sc[tid] = s;
     }

@@ -18,10 +18,11 @@
 //
 // Bound by memory where there is much of it (one MI355X; a copy reaches 4.7 TB/s, 6.9 where the caches hold it):
 //   8192 x 42 cells x 128 channels, float32, forward with residual and relu     97 us for 528 MB    5.4 TB/s
-//   4096 x 42 x 128, bfloat16, with residual and relu     forward 28 us for 132 MB, backward 46 + 4 us for 220 MB    4.7, 4.4 TB/s
+//   4096 x 42 x 128, bfloat16, with residual and relu     forward 29 us for 132 MB, backward 46 + 4 us for 220 MB    4.5, 4.4 TB/s
 //   128 x 42 x 256, float32, as in a training step of the shipped batch         forward 6, backward 8 + 3 us
 //   1 x 42 x 256, float32, one position                                         3.8 us, a launch that does nothing 2.8
-//   61 x 361 x 192, float16, silu     forward 10, backward 15 + 4 us: bound by instructions and the one wave of workgroups
+//   61 x 361 x 192, float16, silu     forward 10.6, backward 15 + 4 us: one workgroup of 1024 a compute unit loads, waits,
+//     computes and stores in turn (0.5 us of the forward pass are the subtraction of x0)
 //   3 x 4096 x 320, bfloat16, silu    5.7 + 7.5 us: two launches, x from the caches the second time
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -316,7 +317,8 @@ k_gn_stats(GnArgs a) {
     gn_put_parts(a, p, s, q, lds);
 }
 
-// 1 / (1 + exp(-z)) by the hardware's 2^x and reciprocal, each good to 2^-23: off by at most (|z| / 2 + 2) 2^-23 of itself
+// 1 / (1 + exp(-z)) by the hardware's 2^x and reciprocal, each good to 2^-23: with log2(e) and its product rounded to 24 bits
+// (1.22 * 2^-24 together) off by at most (0.61 |z| + 2.5) 2^-23 of itself, down to z = -87; what is below 2^-126 may be 0
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
 __device__ __forceinline__ float gn_silu(float z) { return z * gn_sigmoid(z); }
 
@@ -539,7 +541,8 @@ k_gn_bwd_apply(GnArgs a) {
 }
 
 // dw, db: the partial sums of `parts` workgroups, added in a fixed order in 64 bits.  One workgroup: 16 of the 2 C columns.
-// (2 to 4 us.  Not in the launch before it: a counter that finds the last workgroup would have to be kept, and cleared, between calls.)
+// (2 to 4 us.  In the launch before it, whose last workgroup would add the rows up, a counter would be needed that some
+// earlier launch clears: not tried.)
 __global__ void __launch_bounds__(1024)
 k_gn_dparams(const float* __restrict__ dpart, long parts, int first, int C, int wtype, void* dw, void* db) {
     __shared__ double lds[64][17];

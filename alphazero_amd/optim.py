@@ -118,6 +118,10 @@ class FlatAdamW(torch.optim.Optimizer):
     steps are kept in expectation; 12 bytes less traffic and 6 bytes less memory per parameter.  Ranks that hold the
     same weights give the same seed and stay bit-identical.
 
+    Beside the step's own traffic a training loop pays for the views: zero_grad fills the gradients and autograd adds into
+    them, some 16 bytes an element.  In a network of both types every flat buffer spans all parameters: 4 bytes of
+    `flat_g` for each bfloat16 one, 4 of `flat_p16` and `flat_g16` for each float32 one, are never used.
+
     step() may be captured; in a launch that is replayed while a scheduler changes the rate use step_recorded(), as
     with FlatSGD.  The step count lives in device memory (`steps` reads it).  state_dict() is torch.optim.AdamW's
     (exp_avg and exp_avg_sq as the float32 values that the codes stand for, `master` for bfloat16 parameters) and

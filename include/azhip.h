@@ -456,8 +456,9 @@ int  az_sgd_momentum_guarded(float* params, const float* grads, float* momentum_
  * What a residual tower without batch statistics puts where the reference has nn.BatchNorm2d + ReLU
  * (alphazero/models.py:6-28): x [batch][cells][channels] (channels last: a cell's channels lie together),
  *   z = (x - mean) * rstd * weight[c] + bias[c] (+ residual),  y = act(z),
- * mean and rstd = 1 / sqrt(var + eps) over the cells and the channels / groups channels of a sample's group; sums and
- * statistics in 64 bits, the rest in 32, one rounding to the tensors' type.  relu and its gradient pass a NaN on.
+ * mean and rstd = 1 / sqrt(var + eps) over the cells and the channels / groups channels of a sample's group; the statistics
+ * and their sums in 64 bits, the rest in 32 (sums of the backward pass in chains of at most 2048 rows, joined in 64), one
+ * rounding to the tensors' type.  relu and its gradient pass a NaN on.
  * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any alignment (16-byte aligned
  * tensors and groups of a multiple of 4 channels, 8 in 16 bits, run fastest) and any size of up to 2^31 - 1 values a
  * sample, 2^28 channels and 2^32 - 1 work-items in a launch (which tensors of some 10^9 values reach where groups have an
@@ -497,7 +498,8 @@ int  az_group_norm_act_backward(const az_group_norm* g, const void* dy, const vo
  *   p = p * (1 - lr * weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * (with eps 0 an element whose m and v are 0 has no update: the gaps stay zero).
  * p is float32 everywhere; in a run with half != 0 the parameters and gradients are bfloat16 (p16, g16) and p is their
- * master copy, p16 its rounding (a p16 that is not was written by somebody else, and the master becomes it).  state_bits 32: m, v float32.  state_bits 8: m8, v8 one byte per element and
+ * master copy, p16 its rounding (a p16 that is not was written by somebody else, and the master becomes it).
+ * state_bits 32: m, v float32.  state_bits 8: m8, v8 one byte per element and
  * top uint16[blocks][2], 11 leading float bits of each block's largest |m| and v (format and rounding: csrc/az_adamw.hip);
  * they are rounded at random by bits that are a function of (seed, t, element), so the same call gives the same bits
  * on every rank.  step DEVICE int64[AZ_ADAMW_STEPS] counts the updates applied (one counter for each workgroup: set all to
