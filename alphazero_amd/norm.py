@@ -18,17 +18,17 @@ DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _statement(x, num_groups, weight, bias, eps, act, residual):
-    """The same function in torch operations."""
-    rows = x.float().reshape(x.shape[0], num_groups, math.prod(x.shape[1:]) // num_groups)
+    """The same function in torch operations, in 64 bits and rounded once."""
+    rows = x.double().reshape(x.shape[0], num_groups, math.prod(x.shape[1:]) // num_groups)
     var, mean = torch.var_mean(rows, 2, correction=0, keepdim=True)
     z = ((rows - mean) * torch.rsqrt(var + eps)).reshape(x.shape)
     channel = (1, -1) + (1,) * (x.dim() - 2)
     if weight is not None:
-        z = z * weight.float().view(channel)
+        z = z * weight.double().view(channel)
     if bias is not None:
-        z = z + bias.float().view(channel)
+        z = z + bias.double().view(channel)
     if residual is not None:
-        z = z + residual.float()
+        z = z + residual.double()
     if act != 'none':
         z = torch.relu(z) if act == 'relu' else torch.nn.functional.silu(z)
     return z.to(x.dtype)
@@ -48,8 +48,9 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act='relu', 
     float16; residual of x's shape and type; weight and bias [C], both float32 or both of x's type; act 'none', 'relu'
     or 'silu'.  Returns a channels-last tensor of x's type.  Differentiable once with respect to x, weight, bias and
     residual, on the GPU by a backward pass alone: tensors with a forward-mode tangent, torch.func's transforms, batches of
-    gradients and tracing (torch.jit.trace, make_fx, torch.export) are refused there.  Statistics are kept in 64 bits and the sign of a value next to zero, at which relu cuts the gradient, is
-    decided in them; an empty group of values (H * W * C / num_groups == 1) has variance 0."""
+    gradients and tracing (torch.jit.trace, make_fx, torch.export) are refused there.  Statistics are kept in 64 bits and
+    the sign of a value next to zero, at which relu cuts the gradient, is decided in them; a group of one value
+    (H * W * C / num_groups == 1) has variance 0."""
     if act not in ACTS:
         raise ValueError(f"act is 'none', 'relu' or 'silu', got {act!r}")
     if x.dim() not in (2, 4):

@@ -108,3 +108,27 @@ def test_parameter_gradients_are_added_in_chains_of_2048_rows(case):
     if case['batch'] == 1:
         one = 2048 * 256 // 255                    # (an odd number of channels: one to a thread, 256 threads)
     assert rows >= case['batch'] * case['cells'] // one
+
+
+@pytest.mark.parametrize('offset', [0.0, 1e4, 1e6])
+@pytest.mark.parametrize('act', ['none', 'relu', 'silu'])
+def test_the_cpu_statement_keeps_its_statistics_in_64_bits_too(offset, act):
+    """y and the gradients of x, weight, bias and residual against the same formulas on 64-bit inputs: one rounding of each, and
+    what two 64-bit means of `offset` are apart (2^-52 of it), by rstd |w| < 2, for each term."""
+    n, c, groups, h, w = 5, 12, 3, 6, 7
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g)
+    x, wt, b, r, dy = rnd(n, c, h, w) + offset, 1 + 0.3 * rnd(c), 0.3 * rnd(c), rnd(n, c, h, w), rnd(n, c, h, w)
+    leaves = [t.clone().requires_grad_() for t in (x, wt, b, r)]
+    y = group_norm_act(leaves[0], groups, leaves[1], leaves[2], act=act, residual=leaves[3])
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    exact = [t.double().requires_grad_() for t in (x, wt, b, r)]
+    rows = exact[0].reshape(n, groups, -1)
+    centred = rows - rows.mean(2, keepdim=True)
+    z = (centred / torch.sqrt((centred ** 2).mean(2, keepdim=True) + 1e-5)).reshape(x.shape) * exact[1].view(1, c, 1, 1)
+    z = z + exact[2].view(1, c, 1, 1) + exact[3]
+    want_y = {'none': lambda t: t, 'relu': torch.relu, 'silu': torch.nn.functional.silu}[act](z)
+    want = [want_y.detach(), *torch.autograd.grad(want_y, exact, dy.double())]
+    for k, (a, e) in enumerate(zip(got, want)):
+        terms = n * h * w if k in (2, 3) else 4
+        assert bool(((a.double() - e).abs() <= 2.0 ** -24 * (1.01 * e.abs() + 1e-6) + terms * offset * 2.0 ** -51).all()), k
