@@ -50,7 +50,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act='relu', 
     residual, on the GPU by a backward pass alone: tensors with a forward-mode tangent, torch.func's transforms, batches of
     gradients and tracing (torch.jit.trace, make_fx, torch.export) are refused there.  Statistics are kept in 64 bits and
     the sign of a value next to zero, at which relu cuts the gradient, is decided in them; a group of one value
-    (H * W * C / num_groups == 1) has variance 0."""
+    (H * W * C / num_groups == 1) has variance 0.  On the GPU values lie below 2^126 and sqrt(var + eps) between 2^-125 and
+    2^125."""
     if act not in ACTS:
         raise ValueError(f"act is 'none', 'relu' or 'silu', got {act!r}")
     if x.dim() not in (2, 4):

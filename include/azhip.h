@@ -462,7 +462,8 @@ int  az_sgd_momentum_guarded(float* params, const float* grads, float* momentum_
  * x, residual, y, dy, dx, dresidual have one type, weight / bias / dweight / dbias another; any alignment (16-byte aligned
  * tensors and groups of a multiple of 4 channels, 8 in 16 bits, run fastest) and any size of up to 2^31 - 1 values a
  * sample, 2^28 channels and 2^32 - 1 work-items in a launch (which tensors of some 10^9 values reach where groups have an
- * odd number of channels, and of 10^10 otherwise).  A call that needs more is refused before anything is launched.   */
+ * odd number of channels, and of 10^10 otherwise).  A call that needs more is refused before anything is launched.
+ * mean, rstd and x - mean are used in 32 bits: sqrt(var + eps) between 2^-125 and 2^125, values below 2^126.          */
 #define AZ_F32  0
 #define AZ_BF16 1
 #define AZ_F16  2
@@ -484,8 +485,8 @@ int64_t az_group_norm_workspace_bytes(const az_group_norm* g, int32_t backward);
 int  az_group_norm_act(const az_group_norm* g, const void* x, const void* weight, const void* bias, const void* residual,
                        void* y, double* stats, void* workspace, int64_t workspace_bytes, void* stream);
 /* The gradients of sum(dy * y): dx, dweight, dbias, dresidual, each of them written unless NULL.  x, weight, bias,
- * residual and stats as in the forward call.  Sums over the batch are added in a fixed order: the same inputs give the
- * same bits.                                                                                                      */
+ * residual and stats as in the forward call; no output may overlap an input or another output.  Sums over the batch are
+ * added in a fixed order: the same inputs give the same bits.                                                      */
 int  az_group_norm_act_backward(const az_group_norm* g, const void* dy, const void* x, const void* weight, const void* bias,
                                 const void* residual, const double* stats, void* dx, void* dweight, void* dbias,
                                 void* dresidual, void* workspace, int64_t workspace_bytes, void* stream);

@@ -213,3 +213,13 @@ def test_weight_and_bias_off_any_border(dtype, param, shape, act):
     for kw, kb in ((1, 1), (3, 0), (0, 1)):
         got = _run(x, groups, odd(wt, kw), odd(b, kb), r, dy, act)
         assert all(torch.equal(got[k], want[k]) for k in want), (kw, kb)
+
+
+@pytest.mark.parametrize('gain', [2.0 ** 120, 2.0 ** 60, 2.0 ** -60, 2.0 ** -120])
+@pytest.mark.parametrize('shape', [(3, 32, 4, 6, 7), (3, 48, 4, 19, 19), (1, 320, 32, 64, 64)])
+def test_the_ends_of_the_range(shape, gain):
+    n, c, groups, h, w = shape
+    x, wt, b, r, dy = _inputs(n, c, h, w, torch.float32, torch.float32, True, 39, 0.0, gain)
+    for act in ('relu', 'silu'):
+        want, tol = _reference(x, groups, wt, b, r, dy, act, eps=0.0)
+        _check(_run(x, groups, wt, b, r, dy, act, eps=0.0), want, tol, torch.float32, torch.float32)
